@@ -360,6 +360,79 @@ int asm_policy_mlp_act_bf16(int E, int n_a, int obs_dim, int hidden, int act_dim
                             const void *w2, const void *w3, const void *w4, const float *bias, float *act,
                             float noise_scale, float epsilon, uint64_t seed, uint32_t step, int64_t env0, void *stream);
 
+/* ---- Group D: recurrent on-policy training -----------------------------------------------------
+ * A policy with a memory over time, the advantages of an episode and the clipped policy loss.  Device memory throughout,
+ * nothing allocates or synchronises, work is enqueued on `stream`; `ws` is the caller's scratch memory of at least the
+ * size the matching *_workspace function returns (aligned to 16 bytes; NULL where that is 0), free again once the stream
+ * has passed the call; two calls that may run at the same time need two.
+ * dtype: ASM_SEQ_F32 or ASM_SEQ_BF16, the type of gate, x, h and their gradients, or of mean, log_std and theirs; all
+ * other floating arrays are float32.  Strides are in elements.  Outputs must not overlap inputs or each other. */
+#define ASM_SEQ_F32 0
+#define ASM_SEQ_BF16 1
+
+/* Memory over a sequence.  gate, x, h: element (t, b, d) at [t * st + b * sb + d]; per step and channel
+ *     a = sigmoid(gate), h_t = a h_{t-1} + (1 - a) x_t,   h_{-1} = h0 (NULL: zeros),
+ * in float32; h_t is rounded once to dtype where it is stored.  resets (nullable; element (t, b) at [t * r_st + b * r_sb]):
+ * where nonzero, the state in front of step t counts as zero, whatever it holds.  lengths (nullable, [B], clamped to
+ * 0..T): steps from lengths[b] on are not part of the sequence: h is zero there, the state passes.  h_last
+ * (nullable): [B][D], the state behind the last step.  h0, h_last, dh0, dh_last: [B][D] contiguous. */
+int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D);
+int asm_gated_scan_forward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
+                           const void *x, int64_t x_st, int64_t x_sb, const float *h0 /*nullable*/, const uint8_t *resets /*nullable*/,
+                           int64_t r_st, int64_t r_sb, const int32_t *lengths /*nullable*/, void *h, int64_t h_st, int64_t h_sb,
+                           float *h_last /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
+/* Gradients of the above: dh (nullable: zeros) of h, dh_last (nullable: zeros) of h_last.  h: the forward pass's output.
+ * Writes dgate, dx (zero beyond a sequence's length) and dh0 (nullable). */
+int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
+                            const void *x, int64_t x_st, int64_t x_sb, const void *h, int64_t h_st, int64_t h_sb,
+                            const float *h0 /*nullable*/, const uint8_t *resets /*nullable*/, int64_t r_st, int64_t r_sb,
+                            const int32_t *lengths /*nullable*/, const void *dh /*nullable*/, int64_t dh_st, int64_t dh_sb,
+                            const float *dh_last /*nullable*/, void *dgate, int64_t dgate_st, int64_t dgate_sb, void *dx,
+                            int64_t dx_st, int64_t dx_sb, float *dh0 /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
+/* One step of a rollout: state [B][D] float32 is updated in place, out gets the new state in dtype.  Row b of gate, x and
+ * out starts at b * *_sb; reset (nullable): element b at [b * r_sb], nonzero: the state counts as zero first. */
+int asm_gated_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t gate_sb, const void *x, int64_t x_sb,
+                        float *state, const uint8_t *reset /*nullable*/, int64_t r_sb, void *out, int64_t out_sb, void *stream);
+
+/* Advantages and returns of an episode: rewards [T][B][D], values [T + 1][B][D] (a time step contiguous, steps rew_st /
+ * val_st elements apart), dones (nullable, uint8 [T][B][D], done_st): nonzero ends the episode at that step, the value
+ * and the advantage behind it do not count, whatever they hold.  lengths (nullable, [B], clamped to 0..T): row b ends
+ * after lengths[b] steps, with values[lengths[b]] behind its last one; beyond it adv and ret are zero.
+ *     delta = rewards_t + gamma (1 - done) values_{t+1} - values_t,  adv_t = delta + gamma lam (1 - done) adv_{t+1},
+ *     ret_t = adv_t + values_t                                             (adv, ret: [T][B][D] contiguous)
+ * moments (nullable, 2 floats): mean and 1 / (standard deviation + 1e-8) of adv over all steps that are part of an episode
+ * (population deviation), summed in double in a fixed order.  0 <= gamma, lam <= 1. */
+int64_t asm_advantages_workspace(int64_t T, int64_t B, int64_t D);
+int asm_advantages_f32(int64_t T, int64_t B, int64_t D, const float *rewards, int64_t rew_st, const float *values, int64_t val_st,
+                       const uint8_t *dones /*nullable*/, int64_t done_st, const int32_t *lengths /*nullable*/, float gamma,
+                       float lam, float *adv, float *ret, float *moments /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
+
+/* A tensor of the policy operators: element (b, i, j) at p[b * sb + i * sn + j * sa], b < B, i < n, j < A; tensors with one
+ * value per row have no j. */
+typedef struct asm_rows { const void *p; int64_t sb, sn, sa; } asm_rows;
+
+/* Clipped policy loss of a diagonal Gaussian policy over B n rows, with its gradients.  Per row, z = (u - mean) / e^s with
+ * s = log_std, u = actions: log_pi = sum_j(-z^2 / 2 - s - log(2 pi) / 2), q = e^(log_pi - log_pi_old),
+ * A = adv, or (adv - adv_moments[0]) adv_moments[1] where moments are given, D = log_pi_ref - log_pi
+ * (log_pi_ref->p NULL: the old policy is the reference):
+ *     row loss = -min(q A, clip(q, 1 - clip, 1 + clip) A) + kl_coef (e^D - 1 - D) - entropy_coef sum_j(s + log(2 pi e) / 2)
+ * loss = the mean over the rows whose mask (uint8; mask->p NULL: all) is nonzero, 0 if there are none.  What a masked row
+ * holds does not matter.  log_std: mean's shape, or with shared_std A values at p[j * sa].
+ * stats, 6 floats: mean of min(..), of e^D - 1 - D, of the entropy, share of rows the clipping cuts off, mean q, rows.
+ * dmean [B][n][A] and dlog_std ([A] with shared_std, else [B][n][A]), contiguous: the gradients for an upstream
+ * gradient of 1.  Row arithmetic and sums in double, sums in a fixed order.  1 <= A <= 32. */
+int64_t asm_policy_loss_workspace(int64_t rows, int A);
+int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_rows *mean, const asm_rows *log_std,
+                    const asm_rows *actions, const asm_rows *log_pi_old, const asm_rows *log_pi_ref, const asm_rows *adv,
+                    const asm_rows *mask, const float *adv_moments /*nullable*/, double clip, double kl_coef, double entropy_coef,
+                    float *loss, float *stats, void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream);
+/* Multiplies n_mean values of dmean and n_std of dlog_std by *grad (device); reads and writes nothing when that is 1. */
+int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream);
+/* actions = mean + e^log_std noise (noise->p NULL: actions are given, not written) and log_pi of the actions as they are
+ * stored in float32.  A log_std shared by all rows has sb = sn = 0. */
+int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_rows *mean, const asm_rows *log_std, const asm_rows *noise,
+                     const asm_rows *actions, const asm_rows *log_pi, void *stream);
+
 /* Self-test hook: which kernel asm_batch_step_f32 would launch for these arguments: waves per workgroup of the
  * multi-wave kernel (4, 2, 1) or 0 for the generic kernel, plus 16 if its lattice path is taken, plus 32 if the
  * generic kernel's (large swarms), plus 64 if the pair passes go through cell lists, plus 128 for the three-launch

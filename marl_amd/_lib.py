@@ -41,6 +41,13 @@ class AsmLattice(C.Structure):
                 ("xform", C.c_void_p), ("l_cell_min", C.c_double)]
 
 
+class AsmRows(C.Structure):
+    """struct asm_rows of include/marl_amd_env.h (device pointer as an integer, strides in elements)."""
+    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("sn", C.c_int64), ("sa", C.c_int64)]
+
+
+SEQ_F32, SEQ_BF16 = 0, 1
+
 # Every symbol include/marl_amd_env.h declares.
 EXPORTS = ["_get_observation", "_get_reward", "_sf_b2b_all", "_get_dist_b2w", "calculateActionPrior",
            "asm_default_params", "asm_obs_dim", "asm_abi_version", "asm_last_error", "asm_compat_status", "asm_device_count",
@@ -48,7 +55,10 @@ EXPORTS = ["_get_observation", "_get_reward", "_sf_b2b_all", "_get_dist_b2w", "c
            "asm_batch_random_actions_f32", "asm_batch_metrics_f64", "asm_batch_rule_actions_f32", "asm_replay_gather_f32", "asm_replay_draw_indices",
            "asm_debug_sqrt_f64", "asm_debug_cos_f32_max_err", "asm_get_observation_noalloc", "asm_lattice_build",
            "asm_batch_check_lattice", "asm_set_step_schedule", "asm_debug_step_schedule",
-           "asm_policy_mlp_forward_bf16", "asm_policy_mlp_act_bf16", "asm_obs_rows_f32"]
+           "asm_policy_mlp_forward_bf16", "asm_policy_mlp_act_bf16", "asm_obs_rows_f32",
+           "asm_gated_scan_workspace", "asm_gated_scan_forward", "asm_gated_scan_backward", "asm_gated_scan_step",
+           "asm_advantages_workspace", "asm_advantages_f32", "asm_policy_loss_workspace", "asm_policy_loss",
+           "asm_policy_loss_scale", "asm_gaussian_act"]
 
 _lib = None
 
@@ -111,6 +121,28 @@ def load() -> C.CDLL:
     lib.asm_policy_mlp_act_bf16.argtypes = [i32] * 5 + [vp] * 7 + [C.c_float, C.c_float, u64, u32, i64, vp]
     lib.asm_obs_rows_f32.restype = C.c_int
     lib.asm_obs_rows_f32.argtypes = [i32, i32, i32, vp, vp, vp]
+    RP, f32, f64 = C.POINTER(AsmRows), C.c_float, C.c_double
+    lib.asm_gated_scan_workspace.restype = i64
+    lib.asm_gated_scan_workspace.argtypes = [i32, i64, i64, i64]
+    lib.asm_gated_scan_forward.restype = C.c_int
+    lib.asm_gated_scan_forward.argtypes = [i32, i64, i64, i64] + [vp, i64, i64] * 2 + [vp, vp, i64, i64, vp] + [vp, i64, i64] + [vp, vp, i64, vp]
+    lib.asm_gated_scan_backward.restype = C.c_int
+    lib.asm_gated_scan_backward.argtypes = [i32, i64, i64, i64] + [vp, i64, i64] * 3 + [vp, vp, i64, i64, vp] + [vp, i64, i64] + [vp] + \
+        [vp, i64, i64] * 2 + [vp, vp, i64, vp]
+    lib.asm_gated_scan_step.restype = C.c_int
+    lib.asm_gated_scan_step.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp]
+    lib.asm_advantages_workspace.restype = i64
+    lib.asm_advantages_workspace.argtypes = [i64, i64, i64]
+    lib.asm_advantages_f32.restype = C.c_int
+    lib.asm_advantages_f32.argtypes = [i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, f32, f32, vp, vp, vp, vp, i64, vp]
+    lib.asm_policy_loss_workspace.restype = i64
+    lib.asm_policy_loss_workspace.argtypes = [i64, i32]
+    lib.asm_policy_loss.restype = C.c_int
+    lib.asm_policy_loss.argtypes = [i32, i64, i64, i32, i32] + [RP] * 7 + [vp, f64, f64, f64] + [vp] * 5 + [i64, vp]
+    lib.asm_policy_loss_scale.restype = C.c_int
+    lib.asm_policy_loss_scale.argtypes = [i32, vp, i64, vp, i64, vp, vp]
+    lib.asm_gaussian_act.restype = C.c_int
+    lib.asm_gaussian_act.argtypes = [i32, i64, i64, i32] + [RP] * 5 + [vp]
     lib.asm_set_step_schedule.restype = None
     lib.asm_set_step_schedule.argtypes = [C.c_int]
     if lib.asm_abi_version() != ABI_VERSION:

@@ -17,6 +17,7 @@
 #include <mutex>
 
 #include "asm_kernels.h"
+#include "seq_kernels.h"
 
 using asmenv::DevParams;
 
@@ -596,6 +597,156 @@ int asm_policy_mlp_forward_bf16(int E, int n_a, int obs_dim, int hidden, int act
                                 const void *w2, const void *w3, const void *w4, const float *bias, float *act, void *stream)
 {
     return asm_policy_mlp_act_bf16(E, n_a, obs_dim, hidden, act_dim, obs, w1, w2, w3, w4, bias, act, 0.f, 0.f, 0, 0, 0, stream);
+}
+
+// ---- group D: recurrent on-policy training ----
+static int seq_dims(const char *fn, int dtype, int64_t T, int64_t B, int64_t D)
+{
+    if (dtype != ASM_SEQ_F32 && dtype != ASM_SEQ_BF16) return fail(1, "%s: dtype = %d (supported: ASM_SEQ_F32, ASM_SEQ_BF16)", fn, dtype);
+    if (T < 0 || B < 0 || D < 0) return fail(1, "%s: negative size", fn);
+    // (time steps and the threads of a launch are counted in 32 bits, offsets in 64)
+    if (T > (1 << 30) || B > (1 << 30) || D > (1 << 30) || B * D > (1 << 30))
+        return fail(1, "%s: T = %lld, B x D = %lld x %lld: too large", fn, (long long)T, (long long)B, (long long)D);
+    return 0;
+}
+static int seq_ws(const char *fn, const void *ws, int64_t have, int64_t need)
+{
+    if (need > 0 && (!ws || have < need)) return fail(1, "%s: %lld bytes of workspace, %lld needed", fn, (long long)(ws ? have : 0), (long long)need);
+    if (need > 0 && (reinterpret_cast<uintptr_t>(ws) & 15)) return fail(1, "%s: the workspace is not aligned to 16 bytes", fn);
+    return 0;
+}
+
+int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
+{
+    if (seq_dims("asm_gated_scan_workspace", dtype, T, B, D)) return -1;
+    return B * D == 0 ? 0 : asmseq::scan_workspace(dtype, T, B, D);
+}
+
+int asm_gated_scan_forward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
+                           const void *x, int64_t x_st, int64_t x_sb, const float *h0, const uint8_t *resets, int64_t r_st,
+                           int64_t r_sb, const int32_t *lengths, void *h, int64_t h_st, int64_t h_sb, float *h_last, void *ws,
+                           int64_t ws_bytes, void *stream)
+{
+    if (int rc = seq_dims("asm_gated_scan_forward", dtype, T, B, D)) return rc;
+    if (B * D == 0) return 0;
+    if (T > 0 && (!gate || !x || !h)) return fail(1, "asm_gated_scan_forward: NULL pointer");
+    if (int rc = seq_ws("asm_gated_scan_forward", ws, ws_bytes, asmseq::scan_workspace(dtype, T, B, D))) return rc;
+    asmseq::ScanArgs a{};
+    a.dtype = dtype; a.T = T; a.B = B; a.D = D;
+    a.gate = {gate, gate_st, gate_sb}; a.x = {x, x_st, x_sb}; a.h0 = h0;
+    a.resets = resets; a.r_st = r_st; a.r_sb = r_sb; a.lengths = lengths;
+    a.out = {h, h_st, h_sb}; a.h_last = h_last; a.ws = ws;
+    int rc = asmseq::launch_scan_forward(a, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_gated_scan_forward") : 0;
+}
+
+int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
+                            const void *x, int64_t x_st, int64_t x_sb, const void *h, int64_t h_st, int64_t h_sb,
+                            const float *h0, const uint8_t *resets, int64_t r_st, int64_t r_sb, const int32_t *lengths,
+                            const void *dh, int64_t dh_st, int64_t dh_sb, const float *dh_last, void *dgate, int64_t dgate_st,
+                            int64_t dgate_sb, void *dx, int64_t dx_st, int64_t dx_sb, float *dh0, void *ws, int64_t ws_bytes,
+                            void *stream)
+{
+    if (int rc = seq_dims("asm_gated_scan_backward", dtype, T, B, D)) return rc;
+    if (B * D == 0) return 0;
+    if (T > 0 && (!gate || !x || !h || !dgate || !dx)) return fail(1, "asm_gated_scan_backward: NULL pointer");
+    if (int rc = seq_ws("asm_gated_scan_backward", ws, ws_bytes, asmseq::scan_workspace(dtype, T, B, D))) return rc;
+    asmseq::ScanArgs a{};
+    a.dtype = dtype; a.T = T; a.B = B; a.D = D;
+    a.gate = {gate, gate_st, gate_sb}; a.x = {x, x_st, x_sb}; a.h = {h, h_st, h_sb}; a.dh = {dh, dh_st, dh_sb};
+    a.h0 = h0; a.dh_last = dh_last; a.resets = resets; a.r_st = r_st; a.r_sb = r_sb; a.lengths = lengths;
+    a.dgate = {dgate, dgate_st, dgate_sb}; a.dx = {dx, dx_st, dx_sb}; a.dh0 = dh0; a.ws = ws;
+    int rc = asmseq::launch_scan_backward(a, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_gated_scan_backward") : 0;
+}
+
+int asm_gated_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t gate_sb, const void *x, int64_t x_sb,
+                        float *state, const uint8_t *reset, int64_t r_sb, void *out, int64_t out_sb, void *stream)
+{
+    if (int rc = seq_dims("asm_gated_scan_step", dtype, 1, B, D)) return rc;
+    if (B * D == 0) return 0;
+    if (!gate || !x || !state || !out) return fail(1, "asm_gated_scan_step: NULL pointer");
+    int rc = asmseq::launch_scan_step(dtype, B, D, gate, gate_sb, x, x_sb, state, reset, r_sb, out, out_sb, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_gated_scan_step") : 0;
+}
+
+int64_t asm_advantages_workspace(int64_t T, int64_t B, int64_t D)
+{
+    if (seq_dims("asm_advantages_workspace", ASM_SEQ_F32, T, B, D)) return -1;
+    return B * D == 0 ? 0 : asmseq::advantages_workspace(T, B * D);
+}
+
+int asm_advantages_f32(int64_t T, int64_t B, int64_t D, const float *rewards, int64_t rew_st, const float *values, int64_t val_st,
+                       const uint8_t *dones, int64_t done_st, const int32_t *lengths, float gamma, float lam, float *adv,
+                       float *ret, float *moments, void *ws, int64_t ws_bytes, void *stream)
+{
+    if (int rc = seq_dims("asm_advantages_f32", ASM_SEQ_F32, T, B, D)) return rc;
+    if (!(gamma >= 0.f && gamma <= 1.f && lam >= 0.f && lam <= 1.f)) return fail(1, "asm_advantages_f32: gamma and lam must lie in [0, 1]");
+    if (T < 1 || B * D == 0) return fail(1, "asm_advantages_f32: no steps or no rows");
+    if (!rewards || !values || !adv || !ret) return fail(1, "asm_advantages_f32: NULL pointer");
+    if (int rc = seq_ws("asm_advantages_f32", ws, ws_bytes, asmseq::advantages_workspace(T, B * D))) return rc;
+    asmseq::AdvArgs a{T, B * D, D, rewards, values, rew_st, val_st, done_st, dones, lengths, gamma, lam, adv, ret, moments, ws};
+    int rc = asmseq::launch_advantages(a, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_advantages_f32") : 0;
+}
+
+static asmseq::Rows rows_of(const asm_rows *t) { return t ? asmseq::Rows{t->p, t->sb, t->sn, t->sa} : asmseq::Rows{}; }
+static int policy_dims(const char *fn, int dtype, int64_t B, int64_t n, int A)
+{
+    if (int rc = seq_dims(fn, dtype, 1, B, n)) return rc;
+    if (A < 1 || A > 32) return fail(1, "%s: A = %d (supported: 1..32)", fn, A);
+    return 0;
+}
+
+int64_t asm_policy_loss_workspace(int64_t rows, int A)
+{
+    if (policy_dims("asm_policy_loss_workspace", ASM_SEQ_F32, 1, rows, A)) return -1;
+    return asmseq::loss_workspace(rows, A);
+}
+
+int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_rows *mean, const asm_rows *log_std,
+                    const asm_rows *actions, const asm_rows *log_pi_old, const asm_rows *log_pi_ref, const asm_rows *adv,
+                    const asm_rows *mask, const float *adv_moments, double clip, double kl_coef, double entropy_coef, float *loss,
+                    float *stats, void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream)
+{
+    if (int rc = policy_dims("asm_policy_loss", dtype, B, n, A)) return rc;
+    if (!(clip > 0.0 && std::isfinite(clip) && std::isfinite(kl_coef) && std::isfinite(entropy_coef)))
+        return fail(1, "asm_policy_loss: clip must be positive, the coefficients finite");
+    const bool rows = B * n > 0;
+    if (!loss || !stats || (shared_std && (!dlog_std || !log_std || !log_std->p)) ||
+        (rows && (!log_std || !log_std->p || !dmean || !dlog_std || !mean || !mean->p || !actions || !actions->p || !log_pi_old || !log_pi_old->p || !adv || !adv->p)))
+        return fail(1, "asm_policy_loss: NULL pointer");
+    if (int rc = seq_ws("asm_policy_loss", ws, ws_bytes, asmseq::loss_workspace(B * n, A))) return rc;
+    asmseq::LossArgs a{};
+    a.dtype = dtype; a.shared_std = shared_std != 0; a.B = B; a.n = n; a.A = A;
+    a.mean = rows_of(mean); a.log_std = rows_of(log_std); a.actions = rows_of(actions); a.log_pi_old = rows_of(log_pi_old);
+    a.log_pi_ref = rows_of(log_pi_ref); a.adv = rows_of(adv); a.mask = rows_of(mask); a.adv_moments = adv_moments;
+    a.clip = clip; a.kl_coef = kl_coef; a.entropy_coef = entropy_coef;
+    a.loss = loss; a.stats = stats; a.dmean = dmean; a.dlog_std = dlog_std; a.ws = ws;
+    int rc = asmseq::launch_policy_loss(a, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_policy_loss") : 0;
+}
+
+int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream)
+{
+    if (int rc = seq_dims("asm_policy_loss_scale", dtype, 1, n_mean, 1)) return rc;
+    if (n_std < 0 || !grad || (n_mean > 0 && !dmean) || (n_std > 0 && !dlog_std)) return fail(1, "asm_policy_loss_scale: bad arguments");
+    int rc = asmseq::launch_policy_loss_scale(dtype, grad, n_mean, dmean, n_std, dlog_std, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_policy_loss_scale") : 0;
+}
+
+int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_rows *mean, const asm_rows *log_std, const asm_rows *noise,
+                     const asm_rows *actions, const asm_rows *log_pi, void *stream)
+{
+    if (int rc = policy_dims("asm_gaussian_act", dtype, B, n, A)) return rc;
+    if (B * n == 0) return 0;
+    if (!mean || !mean->p || !log_std || !log_std->p || !actions || !actions->p || !log_pi || !log_pi->p)
+        return fail(1, "asm_gaussian_act: NULL pointer");
+    asmseq::ActArgs a{};
+    a.dtype = dtype; a.B = B; a.n = n; a.A = A;
+    a.mean = rows_of(mean); a.log_std = rows_of(log_std); a.noise = rows_of(noise); a.actions = rows_of(actions); a.log_pi = rows_of(log_pi);
+    int rc = asmseq::launch_gaussian_act(a, (hipStream_t)stream);
+    return rc ? hip_fail(rc, "asm_gaussian_act") : 0;
 }
 
 int asm_batch_check_lattice(const asm_params *prm, int E, const float *grid, const int32_t *n_g,

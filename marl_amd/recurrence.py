@@ -1,0 +1,218 @@
+"""First-order recurrences over time on the device (include/marl_amd_env.h, group D): the gated memory of a policy that
+sees only its neighbourhood, over whole sequences with its gradients (gated_scan) and one rollout step at a time
+(gated_scan_step), and the advantages and returns of an episode (advantages).
+
+    a = sigmoid(gate_t),   h_t = a h_{t-1} + (1 - a) x_t
+
+float32 or bfloat16 inputs and outputs, the state itself always float32.  Time-major tensors (T, B, D) are what the rings
+of DeviceReplay hold; batch_first=True takes (B, T, D).  Tensors may be strided as long as their last axis is contiguous
+(others are copied).  No CPU fallback."""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import _lib
+
+_DTYPES = {torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16}
+
+
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise ValueError(msg)
+
+
+def _on_device(fn: str, dev: torch.device, *tensors) -> None:
+    _need(dev.type == "cuda", f"{fn}: the tensors are on {dev}: it runs on a HIP device only")
+    for t in tensors:
+        _need(t is None or t.device == dev, f"{fn}: tensors on different devices")
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(-1) == 1 or t.shape[-1] <= 1 else t.contiguous()
+
+
+def _tb(t: Optional[torch.Tensor], batch_first: bool) -> Tuple[Optional[int], int, int]:
+    """(pointer, stride of time, stride of the batch)"""
+    if t is None:
+        return None, 0, 0
+    s = t.stride()
+    return (t.data_ptr(), s[1], s[0]) if batch_first else (t.data_ptr(), s[0], s[1])
+
+
+def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
+
+
+def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
+    """A leaf's accumulation node belongs to the stream it was first used on and lives as long as any graph that uses the
+    leaf; a backward pass captured into a HIP graph would have to join that other stream, which ends the process.
+    The node remembers its stream (in its own metadata, gone with the node), and such a capture is refused."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    for node, _ in out.grad_fn.next_functions:
+        if type(node).__name__ == "AccumulateGrad":
+            first = node.metadata.setdefault("marl_amd_stream", stream)
+            if first != stream and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("captured into a HIP graph while an autograd graph of the same leaf tensor, made on another stream, is alive: "
+                                   "drop it (its loss and outputs) before capturing")
+    return out
+
+
+def _check_scan(gate, x, h0, resets, lengths, batch_first):
+    fn = "gated_scan"
+    _need(gate.dim() == 3 and gate.shape == x.shape, f"{fn}: gate and x must have one shape of three axes, got {tuple(gate.shape)} and {tuple(x.shape)}")
+    _need(gate.dtype in _DTYPES and x.dtype == gate.dtype, f"{fn}: gate and x must both be float32 or bfloat16, got {gate.dtype} and {x.dtype}")
+    T, B, D = (gate.shape[1], gate.shape[0], gate.shape[2]) if batch_first else gate.shape
+    _need(h0 is None or (h0.shape == (B, D) and h0.dtype == torch.float32), f"{fn}: h0 must be a float32 tensor of shape {(B, D)}")
+    _need(resets is None or (resets.shape == gate.shape[:2] and resets.dtype in (torch.bool, torch.uint8)),
+          f"{fn}: resets must be a bool or uint8 tensor of shape {tuple(gate.shape[:2])}")
+    _need(lengths is None or (lengths.shape == (B,) and lengths.dtype == torch.int32), f"{fn}: lengths must be an int32 tensor of shape {(B,)}")
+    _on_device(fn, gate.device, x, h0, resets, lengths)
+    return T, B, D
+
+
+def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D):
+    lib = _lib.load()
+    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
+    last = torch.empty(B, D, dtype=torch.float32, device=gate.device)
+    dt = _DTYPES[gate.dtype]
+    with torch.cuda.device(gate.device):
+        need = lib.asm_gated_scan_workspace(dt, T, B, D)
+        ws = _workspace(need, gate.device)
+        rc = lib.asm_gated_scan_forward(dt, T, B, D, *_tb(gate, batch_first), *_tb(x, batch_first), _ptr(h0), *_tb(resets, batch_first),
+                                        _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(ws), max(need, 0),
+                                        torch.cuda.current_stream(gate.device).cuda_stream)
+    _lib.check(rc, "asm_gated_scan_forward")
+    return h, last
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, gate, x, h0, resets, lengths, batch_first, dims):
+        ctx.set_materialize_grads(False)
+        h, last = _scan_forward(gate, x, h0, resets, lengths, batch_first, *dims)
+        ctx.save_for_backward(gate, x, h, h0, resets, lengths)
+        ctx.batch_first, ctx.dims = batch_first, dims
+        return h, last
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh, dlast):
+        gate, x, h, h0, resets, lengths = ctx.saved_tensors
+        T, B, D = ctx.dims
+        bf, dev = ctx.batch_first, gate.device
+        lib = _lib.load()
+        dh = None if dh is None else _dense(dh)
+        dlast = None if dlast is None else dlast.contiguous()
+        dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+        dx = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+        dh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
+        dt = _DTYPES[gate.dtype]
+        with torch.cuda.device(dev):
+            need = lib.asm_gated_scan_workspace(dt, T, B, D)
+            ws = _workspace(need, dev)
+            rc = lib.asm_gated_scan_backward(dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf),
+                                             _ptr(lengths), *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0),
+                                             _ptr(ws), max(need, 0), torch.cuda.current_stream(dev).cuda_stream)
+        _lib.check(rc, "asm_gated_scan_backward")
+        return dgate, dx, dh0, None, None, None, None
+
+
+def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *, resets: Optional[torch.Tensor] = None,
+               lengths: Optional[torch.Tensor] = None, batch_first: bool = False) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The memory over a sequence: (h, h_last), h of gate's shape and type, h_last (B, D) float32, the state behind the
+    last step.  Differentiable (once) in gate, x and h0.
+
+    gate, x: (T, B, D), or (B, T, D) with batch_first; float32 or bfloat16, both the same.  h0: (B, D) float32, the state in
+    front of the first step (None: zeros).  resets: bool or uint8 of gate's first two axes; where set, the state counts as
+    zero in front of that step, whatever it holds, and no gradient passes.  lengths: (B,) int32, clamped to 0..T: steps from
+    there on are no part of the sequence; h and the gradients are zero there, and what gate and x hold does not matter.
+    Sequences may be of length 0."""
+    T, B, D = _check_scan(gate, x, h0, resets, lengths, batch_first)
+    gate, x = _dense(gate), _dense(x)
+    h0 = None if h0 is None else h0.contiguous()
+    lengths = None if lengths is None else lengths.contiguous()
+    if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
+        h, last = _GatedScan.apply(gate, x, h0, resets, lengths, batch_first, (T, B, D))
+        return _guard_leaves(h, h.device), last
+    return _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D)
+
+
+def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, reset: Optional[torch.Tensor] = None,
+                    out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One step of the memory in a rollout, without gradients: state (B, D) float32, contiguous, is updated in place, the
+    new state is returned in gate's type (in `out` if given; it may be gate or x itself, not the state).  reset: (B,) bool or uint8; where
+    set, the state counts as zero first."""
+    fn = "gated_scan_step"
+    _need(gate.dim() == 2 and gate.shape == x.shape == state.shape, f"{fn}: gate, x and state must have one shape of two axes")
+    _need(gate.dtype in _DTYPES and x.dtype == gate.dtype, f"{fn}: gate and x must both be float32 or bfloat16, got {gate.dtype} and {x.dtype}")
+    _need(state.dtype == torch.float32 and state.is_contiguous(), f"{fn}: state must be a contiguous float32 tensor")
+    _need(not (state.requires_grad and torch.is_grad_enabled()), f"{fn}: the state is updated in place and cannot require a gradient")
+    B, D = gate.shape
+    _need(reset is None or (reset.shape == (B,) and reset.dtype in (torch.bool, torch.uint8)), f"{fn}: reset must be a bool or uint8 tensor of shape {(B,)}")
+    _need(out is None or (out.shape == gate.shape and out.dtype == gate.dtype and (D <= 1 or out.stride(1) == 1) and (B <= 1 or out.stride(0) >= D)
+                          and not (out.requires_grad and torch.is_grad_enabled())),
+          f"{fn}: out must be a tensor of gate's shape and type with contiguous rows that do not overlap")
+    dev = gate.device
+    _on_device(fn, dev, x, state, reset, out)
+    gate, x = _dense(gate), _dense(x)
+    if out is None:
+        out = torch.empty(B, D, dtype=gate.dtype, device=dev)
+    _need(B * D == 0 or out.data_ptr() != state.data_ptr(), f"{fn}: out and state must be two tensors")
+    with torch.cuda.device(dev):
+        rc = _lib.load().asm_gated_scan_step(_DTYPES[gate.dtype], B, D, gate.data_ptr(), gate.stride(0), x.data_ptr(), x.stride(0), state.data_ptr(),
+                                             _ptr(reset), 0 if reset is None else reset.stride(0), out.data_ptr(), out.stride(0),
+                                             torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "asm_gated_scan_step")
+    torch.autograd.graph.increment_version([state, out])                # (written behind autograd's back)
+    return out
+
+
+def _time_rows(t: torch.Tensor) -> torch.Tensor:
+    """t with every time step contiguous (steps may lie any distance apart)."""
+    return t if t.shape[0] == 0 or t[0].is_contiguous() else t.contiguous()
+
+
+@torch.no_grad()
+def advantages(rewards: torch.Tensor, values: torch.Tensor, *, dones: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
+               gamma: float = 0.95, lam: float = 0.95, moments: bool = False):
+    """Advantages and returns of an episode, without gradients: (adv, ret), or (adv, ret, moments).
+
+        delta_t = r_t + gamma (1 - done_t) V_{t+1} - V_t,   adv_t = delta_t + gamma lam (1 - done_t) adv_{t+1},   ret_t = adv_t + V_t
+
+    rewards: (T, E, ...) float32, T >= 1, for instance DeviceReplay.rew_ring[slot]; values: (T + 1, E, ...) float32, the last
+    one behind the last step; dones: bool or uint8 of rewards' shape: where set, nothing behind that step counts, whatever it holds.
+    lengths: (E,) int32, clamped to 0..T: environment e ends after lengths[e] steps, values[lengths[e]] behind its last one;
+    beyond it both results are zero.  moments=True also returns the two numbers clipped_policy_loss normalises with:
+    mean and 1 / (standard deviation + 1e-8) of the advantages of all steps (population deviation), as a float32 tensor."""
+    fn = "advantages"
+    _need(rewards.dim() >= 2 and rewards.shape[0] >= 1 and rewards.numel() > 0, f"{fn}: rewards must be a non-empty (T, E, ...) tensor")
+    T, E = rewards.shape[0], rewards.shape[1]
+    _need(tuple(values.shape) == (T + 1,) + tuple(rewards.shape[1:]), f"{fn}: values must have the shape {(T + 1,) + tuple(rewards.shape[1:])}")
+    _need(rewards.dtype == torch.float32 and values.dtype == torch.float32, f"{fn}: rewards and values must be float32")
+    _need(dones is None or (dones.shape == rewards.shape and dones.dtype in (torch.bool, torch.uint8)), f"{fn}: dones must be a bool or uint8 tensor of rewards' shape")
+    _need(lengths is None or (lengths.shape == (E,) and lengths.dtype == torch.int32), f"{fn}: lengths must be an int32 tensor of shape {(E,)}")
+    _need(0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0, f"{fn}: gamma and lam must lie in [0, 1]")
+    dev = rewards.device
+    _on_device(fn, dev, values, dones, lengths)
+    rewards, values = _time_rows(rewards), _time_rows(values)
+    dones = None if dones is None else _time_rows(dones)
+    lengths = None if lengths is None else lengths.contiguous()
+    adv = torch.empty(rewards.shape, dtype=torch.float32, device=dev)
+    ret = torch.empty(rewards.shape, dtype=torch.float32, device=dev)
+    mom = torch.empty(2, dtype=torch.float32, device=dev) if moments else None
+    D = rewards[0].numel() // E
+    lib = _lib.load()
+    with torch.cuda.device(dev):
+        need = lib.asm_advantages_workspace(T, E, D)
+        ws = _workspace(need, dev)
+        rc = lib.asm_advantages_f32(T, E, D, rewards.data_ptr(), rewards.stride(0), values.data_ptr(), values.stride(0), _ptr(dones),
+                                    0 if dones is None else dones.stride(0), _ptr(lengths), float(gamma), float(lam), adv.data_ptr(),
+                                    ret.data_ptr(), _ptr(mom), _ptr(ws), max(need, 0), torch.cuda.current_stream(dev).cuda_stream)
+    _lib.check(rc, "asm_advantages_f32")
+    return (adv, ret, mom) if moments else (adv, ret)
