@@ -410,28 +410,28 @@ int asm_advantages_f32(int64_t T, int64_t B, int64_t D, const float *rewards, in
 /* A tensor of the policy operators: element (b, i, j) at p[b * sb + i * sn + j * sa], b < B, i < n, j < A; tensors with one
  * value per row have no j. */
 typedef struct asm_rows { const void *p; int64_t sb, sn, sa; } asm_rows;
+typedef struct asm_loss_rows { asm_rows mean, log_std, actions, log_pi_old, log_pi_ref /*p nullable*/, adv, mask /*p nullable*/; } asm_loss_rows;
+typedef struct asm_act_rows { asm_rows mean, log_std, noise /*p nullable*/, actions, log_pi; } asm_act_rows;
 
 /* Clipped policy loss of a diagonal Gaussian policy over B n rows, with its gradients.  Per row, z = (u - mean) / e^s with
  * s = log_std, u = actions: log_pi = sum_j(-z^2 / 2 - s - log(2 pi) / 2), q = e^(log_pi - log_pi_old),
  * A = adv, or (adv - adv_moments[0]) adv_moments[1] where moments are given, D = log_pi_ref - log_pi
- * (log_pi_ref->p NULL: the old policy is the reference):
+ * (log_pi_ref.p NULL: the old policy is the reference):
  *     row loss = -min(q A, clip(q, 1 - clip, 1 + clip) A) + kl_coef (e^D - 1 - D) - entropy_coef sum_j(s + log(2 pi e) / 2)
- * loss = the mean over the rows whose mask (uint8; mask->p NULL: all) is nonzero, 0 if there are none.  What a masked row
+ * loss = the mean over the rows whose mask (uint8; mask.p NULL: all) is nonzero, 0 if there are none.  What a masked row
  * holds does not matter.  log_std: mean's shape, or with shared_std A values at p[j * sa].
  * stats, 6 floats: mean of min(..), of e^D - 1 - D, of the entropy, share of rows the clipping cuts off, mean q, rows.
  * dmean [B][n][A] and dlog_std ([A] with shared_std, else [B][n][A]), contiguous: the gradients for an upstream
  * gradient of 1.  Row arithmetic and sums in double, sums in a fixed order.  1 <= A <= 32. */
 int64_t asm_policy_loss_workspace(int64_t rows, int A);
-int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_rows *mean, const asm_rows *log_std,
-                    const asm_rows *actions, const asm_rows *log_pi_old, const asm_rows *log_pi_ref, const asm_rows *adv,
-                    const asm_rows *mask, const float *adv_moments /*nullable*/, double clip, double kl_coef, double entropy_coef,
-                    float *loss, float *stats, void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream);
+int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_loss_rows *rows,
+                    const float *adv_moments /*nullable*/, double clip, double kl_coef, double entropy_coef, float *loss, float *stats,
+                    void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream);
 /* Multiplies n_mean values of dmean and n_std of dlog_std by *grad (device); reads and writes nothing when that is 1. */
 int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream);
-/* actions = mean + e^log_std noise (noise->p NULL: actions are given, not written) and log_pi of the actions as they are
+/* actions = mean + e^log_std noise (noise.p NULL: actions are given, not written) and log_pi of the actions as they are
  * stored in float32.  A log_std shared by all rows has sb = sn = 0. */
-int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_rows *mean, const asm_rows *log_std, const asm_rows *noise,
-                     const asm_rows *actions, const asm_rows *log_pi, void *stream);
+int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_act_rows *rows, void *stream);
 
 /* Self-test hook: which kernel asm_batch_step_f32 would launch for these arguments: waves per workgroup of the
  * multi-wave kernel (4, 2, 1) or 0 for the generic kernel, plus 16 if its lattice path is taken, plus 32 if the

@@ -41,11 +41,6 @@ class AsmLattice(C.Structure):
                 ("xform", C.c_void_p), ("l_cell_min", C.c_double)]
 
 
-class AsmRows(C.Structure):
-    """struct asm_rows of include/marl_amd_env.h (device pointer as an integer, strides in elements)."""
-    _fields_ = [("p", C.c_void_p), ("sb", C.c_int64), ("sn", C.c_int64), ("sa", C.c_int64)]
-
-
 SEQ_F32, SEQ_BF16 = 0, 1
 
 # Every symbol include/marl_amd_env.h declares.
@@ -121,7 +116,7 @@ def load() -> C.CDLL:
     lib.asm_policy_mlp_act_bf16.argtypes = [i32] * 5 + [vp] * 7 + [C.c_float, C.c_float, u64, u32, i64, vp]
     lib.asm_obs_rows_f32.restype = C.c_int
     lib.asm_obs_rows_f32.argtypes = [i32, i32, i32, vp, vp, vp]
-    RP, f32, f64 = C.POINTER(AsmRows), C.c_float, C.c_double
+    f32, f64 = C.c_float, C.c_double
     lib.asm_gated_scan_workspace.restype = i64
     lib.asm_gated_scan_workspace.argtypes = [i32, i64, i64, i64]
     lib.asm_gated_scan_forward.restype = C.c_int
@@ -138,11 +133,12 @@ def load() -> C.CDLL:
     lib.asm_policy_loss_workspace.restype = i64
     lib.asm_policy_loss_workspace.argtypes = [i64, i32]
     lib.asm_policy_loss.restype = C.c_int
-    lib.asm_policy_loss.argtypes = [i32, i64, i64, i32, i32] + [RP] * 7 + [vp, f64, f64, f64] + [vp] * 5 + [i64, vp]
+    # (struct asm_loss_rows, asm_act_rows: 7 and 5 times four 64-bit words, passed as packed bytes)
+    lib.asm_policy_loss.argtypes = [i32, i64, i64, i32, i32, vp, vp, f64, f64, f64] + [vp] * 5 + [i64, vp]
     lib.asm_policy_loss_scale.restype = C.c_int
     lib.asm_policy_loss_scale.argtypes = [i32, vp, i64, vp, i64, vp, vp]
     lib.asm_gaussian_act.restype = C.c_int
-    lib.asm_gaussian_act.argtypes = [i32, i64, i64, i32] + [RP] * 5 + [vp]
+    lib.asm_gaussian_act.argtypes = [i32, i64, i64, i32, vp, vp]
     lib.asm_set_step_schedule.restype = None
     lib.asm_set_step_schedule.argtypes = [C.c_int]
     if lib.asm_abi_version() != ABI_VERSION:

@@ -690,7 +690,7 @@ int asm_advantages_f32(int64_t T, int64_t B, int64_t D, const float *rewards, in
     return rc ? hip_fail(rc, "asm_advantages_f32") : 0;
 }
 
-static asmseq::Rows rows_of(const asm_rows *t) { return t ? asmseq::Rows{t->p, t->sb, t->sn, t->sa} : asmseq::Rows{}; }
+static asmseq::Rows rows_of(const asm_rows &t) { return {t.p, t.sb, t.sn, t.sa}; }
 static int policy_dims(const char *fn, int dtype, int64_t B, int64_t n, int A)
 {
     if (int rc = seq_dims(fn, dtype, 1, B, n)) return rc;
@@ -704,23 +704,21 @@ int64_t asm_policy_loss_workspace(int64_t rows, int A)
     return asmseq::loss_workspace(rows, A);
 }
 
-int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_rows *mean, const asm_rows *log_std,
-                    const asm_rows *actions, const asm_rows *log_pi_old, const asm_rows *log_pi_ref, const asm_rows *adv,
-                    const asm_rows *mask, const float *adv_moments, double clip, double kl_coef, double entropy_coef, float *loss,
+int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_loss_rows *t, const float *adv_moments, double clip, double kl_coef, double entropy_coef, float *loss,
                     float *stats, void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream)
 {
     if (int rc = policy_dims("asm_policy_loss", dtype, B, n, A)) return rc;
     if (!(clip > 0.0 && std::isfinite(clip) && std::isfinite(kl_coef) && std::isfinite(entropy_coef)))
         return fail(1, "asm_policy_loss: clip must be positive, the coefficients finite");
     const bool rows = B * n > 0;
-    if (!loss || !stats || (shared_std && (!dlog_std || !log_std || !log_std->p)) ||
-        (rows && (!log_std || !log_std->p || !dmean || !dlog_std || !mean || !mean->p || !actions || !actions->p || !log_pi_old || !log_pi_old->p || !adv || !adv->p)))
+    if (!t || !loss || !stats || (shared_std && (!dlog_std || !t->log_std.p)) ||
+        (rows && (!t->log_std.p || !dmean || !dlog_std || !t->mean.p || !t->actions.p || !t->log_pi_old.p || !t->adv.p)))
         return fail(1, "asm_policy_loss: NULL pointer");
     if (int rc = seq_ws("asm_policy_loss", ws, ws_bytes, asmseq::loss_workspace(B * n, A))) return rc;
     asmseq::LossArgs a{};
     a.dtype = dtype; a.shared_std = shared_std != 0; a.B = B; a.n = n; a.A = A;
-    a.mean = rows_of(mean); a.log_std = rows_of(log_std); a.actions = rows_of(actions); a.log_pi_old = rows_of(log_pi_old);
-    a.log_pi_ref = rows_of(log_pi_ref); a.adv = rows_of(adv); a.mask = rows_of(mask); a.adv_moments = adv_moments;
+    a.mean = rows_of(t->mean); a.log_std = rows_of(t->log_std); a.actions = rows_of(t->actions); a.log_pi_old = rows_of(t->log_pi_old);
+    a.log_pi_ref = rows_of(t->log_pi_ref); a.adv = rows_of(t->adv); a.mask = rows_of(t->mask); a.adv_moments = adv_moments;
     a.clip = clip; a.kl_coef = kl_coef; a.entropy_coef = entropy_coef;
     a.loss = loss; a.stats = stats; a.dmean = dmean; a.dlog_std = dlog_std; a.ws = ws;
     int rc = asmseq::launch_policy_loss(a, (hipStream_t)stream);
@@ -735,16 +733,15 @@ int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dm
     return rc ? hip_fail(rc, "asm_policy_loss_scale") : 0;
 }
 
-int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_rows *mean, const asm_rows *log_std, const asm_rows *noise,
-                     const asm_rows *actions, const asm_rows *log_pi, void *stream)
+int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_act_rows *t, void *stream)
 {
     if (int rc = policy_dims("asm_gaussian_act", dtype, B, n, A)) return rc;
     if (B * n == 0) return 0;
-    if (!mean || !mean->p || !log_std || !log_std->p || !actions || !actions->p || !log_pi || !log_pi->p)
+    if (!t || !t->mean.p || !t->log_std.p || !t->actions.p || !t->log_pi.p)
         return fail(1, "asm_gaussian_act: NULL pointer");
     asmseq::ActArgs a{};
     a.dtype = dtype; a.B = B; a.n = n; a.A = A;
-    a.mean = rows_of(mean); a.log_std = rows_of(log_std); a.noise = rows_of(noise); a.actions = rows_of(actions); a.log_pi = rows_of(log_pi);
+    a.mean = rows_of(t->mean); a.log_std = rows_of(t->log_std); a.noise = rows_of(t->noise); a.actions = rows_of(t->actions); a.log_pi = rows_of(t->log_pi);
     int rc = asmseq::launch_gaussian_act(a, (hipStream_t)stream);
     return rc ? hip_fail(rc, "asm_gaussian_act") : 0;
 }

@@ -7,11 +7,13 @@
 //   loss = mean of L_r over the rows the mask leaves (no rows: 0, and so are the gradients)
 //   dL_r / dlog_pi = (cut ? 0 : -q A) - kl (e^D - 1),   cut = A > 0 and q > 1 + eps, or A < 0 and q < 1 - eps
 //   dmu_j = dL/dlog_pi z_j e^-s_j,      ds_j = dL/dlog_pi (z_j^2 - 1) - ent
-// The arithmetic of a row is in double: whether a ratio lies beyond the clipping border decides between a gradient and
-// none, and e^D - 1 - D cancels for nearly equal policies (the CU's double rate equals its float rate, and the rows are
-// bound by their bytes).  The gradients are written in the same pass as the loss: a mean over rows needs only their
-// count, known without a mask and counted ahead with one.  Sums: per thread in double, per workgroup in a fixed order,
-// then over the workgroups in a fixed order: the same inputs give the same bits.
+// What is in double and what is not: z, log_pi, d and q = e^d are in double, and so is the decision whether a ratio lies beyond the
+// clipping border (d against log(1 +- eps): it decides between a gradient and none) and the sum of the gains, whose terms
+// cancel.  e^D - 1 - D, which cancels for nearly equal policies, is its own series where |D| < 1, in float32; so are the
+// products behind the row's gradient.  Sums are in double.
+// The gradients are written in the same pass as the loss: a mean over rows needs only their count, known without a mask
+// and counted ahead with one.  Sums: per thread, per workgroup in a fixed order, then over the workgroups in a fixed order:
+// the same inputs give the same bits.
 
 constexpr int LOSS_SUMS = 5;                                            // gain, KL, entropy, cut rows, ratio; then A sums of ds
 
@@ -20,7 +22,7 @@ struct LossDev {
     int A;
     Rows mean, log_std, actions, old, ref, adv, mask;
     const float *moments;
-    double lo, hi, kl, ent;
+    double lo, hi, dlo, dhi, kl, ent;                                   // 1 -+ clip and their logarithms
     float *loss, *stats;
     void *dmean, *dstd;
     double *part;                                                       // [LOSS_SUMS + A][workgroups]
@@ -65,18 +67,58 @@ template <typename TM, bool SHARED> __device__ __forceinline__ void loss_finish(
     if (SHARED && threadIdx.x < (unsigned)p.A) reinterpret_cast<TM *>(p.dstd)[threadIdx.x] = from_float<TM>((float)tot[LOSS_SUMS + threadIdx.x]);
 }
 
+// e^x and e^-x in double for |x| < 700 (beyond: infinite or 0): x = n log 2 + r, |r| <= log(2) / 2, the even and the odd part of
+// e^r's series up to r^13 (the next term is below 1e-17), their sum and difference scaled by 2^n and 2^-n.
+__device__ __forceinline__ void exp_both(double x, double &ep, double &em)
+{
+    const double c = x > 800.0 ? 800.0 : x < -800.0 ? -800.0 : x;       // (NaN stays)
+    const double n = __builtin_rint(c * 1.44269504088896340736), r = __fma_rn(n, -1.9082149292705877e-10, __fma_rn(n, -0.69314718036912381649, c)), s = r * r;
+    double e = 1.0 / 479001600.0, o = 1.0 / 6227020800.0;
+    e = __fma_rn(e, s, 1.0 / 3628800.0); o = __fma_rn(o, s, 1.0 / 39916800.0);
+    e = __fma_rn(e, s, 1.0 / 40320.0);   o = __fma_rn(o, s, 1.0 / 362880.0);
+    e = __fma_rn(e, s, 1.0 / 720.0);     o = __fma_rn(o, s, 1.0 / 5040.0);
+    e = __fma_rn(e, s, 1.0 / 24.0);      o = __fma_rn(o, s, 1.0 / 120.0);
+    e = __fma_rn(e, s, 0.5);             o = __fma_rn(o, s, 1.0 / 6.0);
+    e = __fma_rn(e, s, 1.0);             o = __fma_rn(o, s, 1.0) * r;
+    const int k = (int)n;
+    ep = __builtin_ldexp(e + o, k);
+    em = __builtin_ldexp(e - o, -k);
+}
+
+// k = e^x - 1 - x and em = e^x - 1, e = e^x given.  |x| < 1: x^2 (1/2! + x/3! + ... + x^9/11!), the rest below 2^-28 of it;
+// beyond, e^x - 1 - x loses at most a factor (e + 1 + |x|) / k < 8 of the rounding.
+__device__ __forceinline__ void expm1_parts(float x, float e, float &k, float &em)
+{
+    float s = 2.5052108385441718775e-8f;                                // 1/11!
+    s = __fmaf_rn(s, x, 2.7557319223985890653e-7f);
+    s = __fmaf_rn(s, x, 2.7557319223985892511e-6f);
+    s = __fmaf_rn(s, x, 2.4801587301587301566e-5f);
+    s = __fmaf_rn(s, x, 1.9841269841269841253e-4f);
+    s = __fmaf_rn(s, x, 1.3888888888888889419e-3f);
+    s = __fmaf_rn(s, x, 8.3333333333333332177e-3f);
+    s = __fmaf_rn(s, x, 4.1666666666666664354e-2f);
+    s = __fmaf_rn(s, x, 1.6666666666666665741e-1f);
+    s = __fmaf_rn(s, x, 0.5f);
+    const float small = s * x * x;
+    const bool near = fabsf(x) < 1.f;
+    em = near ? x + small : e - 1.f;
+    k = near ? small : em - x;
+}
+
 // A row is worked on by GL neighbouring lanes, AM components each (lane `sub` of them has components sub AM .. sub AM + AM - 1):
 // one lane up to four components, more lanes beyond, so that no variant keeps more than four components' values in
-// registers.  SHARED: one log_std for all rows.  PACKED: A == GL AM and the rows of mean (and log_std) are contiguous and
-// aligned to AM values: one load each.
-template <typename TM, int AM, int GL, bool SHARED, bool PACKED, int BS>
+// registers.  SHARED: one log_std for all rows.  LINEAR: every tensor but the actions has its rows one behind the other
+// (mean and log_std A == GL AM values apart and aligned to AM of them, the others one): a row's address is the uniform base
+// of the workgroup's rows and the thread's number, and takes no vector instruction.  Otherwise each tensor's offset is walked
+// along by additions.  A workgroup has a contiguous piece of the rows; the next row's values are in flight while one is worked on.
+template <typename TM, int AM, int GL, bool SHARED, bool LINEAR, int BS>
 __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
 {
     constexpr int K = LOSS_SUMS + (SHARED ? AM * GL : 0), ROWS = BS / GL;
     __shared__ double sh_s[AM * GL], sh_e[AM * GL], red[BS / 64][K], tot[K];
     __shared__ int64_t sh_c[BS / 64];
     const int tid = threadIdx.x, sub = GL > 1 ? tid & (GL - 1) : 0, j0 = sub * AM;
-    const bool masked = p.mask.p != nullptr;
+    const bool masked = p.mask.p != nullptr, own_ref = p.ref.p != p.old.p;
     const uint8_t *maskp = reinterpret_cast<const uint8_t *>(p.mask.p);
     if (SHARED && tid < p.A) {
         const double s = (double)to_float(reinterpret_cast<const TM *>(p.log_std.p)[tid * p.log_std.sa]);
@@ -93,62 +135,105 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
         count = block_count<BS>(c, sh_c);
     }
     __syncthreads();
-    const double w = 1.0 / (double)(count > 0 ? count : 1);
+    const double wd = 1.0 / (double)(count > 0 ? count : 1);
+    const float w = (float)wd, klf = (float)p.kl, entw = (float)(p.ent * wd);
     double am = 0.0, ar = 1.0;
     if (p.moments) { am = (double)p.moments[0]; ar = (double)p.moments[1]; }
     double sum[LOSS_SUMS + AM];
 #pragma unroll
     for (int k = 0; k < LOSS_SUMS + AM; ++k) sum[k] = 0.0;
 
-    // The element offsets of a thread's row in each tensor move on by additions: the division and the products of an
-    // address are paid once per thread.
-    const int64_t stride = (int64_t)gridDim.x * ROWS, db = stride / p.n, di = stride - db * p.n;
-    int64_t r = (int64_t)blockIdx.x * ROWS + tid / GL, b0 = r / p.n, i = r - b0 * p.n;
-    int64_t o_mean = b0 * p.mean.sb + i * p.mean.sn + j0 * p.mean.sa, o_act = b0 * p.actions.sb + i * p.actions.sn + j0 * p.actions.sa,
-            o_old = b0 * p.old.sb + i * p.old.sn, o_ref = b0 * p.ref.sb + i * p.ref.sn, o_adv = b0 * p.adv.sb + i * p.adv.sn,
-            o_mask = b0 * p.mask.sb + i * p.mask.sn, o_std = b0 * p.log_std.sb + i * p.log_std.sn + j0 * p.log_std.sa;
-    // (the GL lanes of a row leave the loop together)
-    for (; r < p.rows; r += stride) {
-        const bool valid = !masked || maskp[o_mask] != 0;
-        float mu[AM], u[AM], sd[AM];
-        if (PACKED) {
-            load_vec<TM, AM>(mu, p.mean.p, o_mean);
-            if (!SHARED) load_vec<TM, AM>(sd, p.log_std.p, o_std);
+    // this workgroup's rows: [first, last)
+    const int64_t first = p.rows * blockIdx.x / gridDim.x, last = p.rows * (blockIdx.x + 1) / gridDim.x;
+    const int lane_row = tid / GL;
+    const int64_t db = ROWS / p.n, di = ROWS - db * p.n;                // (uniform)
+    int64_t b0 = (first + lane_row) / p.n, i = first + lane_row - b0 * p.n;
+    int64_t o_act = b0 * p.actions.sb + i * p.actions.sn + j0 * p.actions.sa;
+    int64_t o_mean = 0, o_old = 0, o_ref = 0, o_adv = 0, o_mask = 0, o_std = 0;
+    if (!LINEAR) {
+        o_mean = b0 * p.mean.sb + i * p.mean.sn + j0 * p.mean.sa; o_old = b0 * p.old.sb + i * p.old.sn; o_ref = b0 * p.ref.sb + i * p.ref.sn;
+        o_adv = b0 * p.adv.sb + i * p.adv.sn; o_mask = b0 * p.mask.sb + i * p.mask.sn; o_std = b0 * p.log_std.sb + i * p.log_std.sn + j0 * p.log_std.sa;
+    }
+    struct Raw { Pack<TM, AM> mu, sd; float u[AM], old, ref, adv; uint8_t ok; };
+    auto fetch_row = [&](Raw &x, int64_t base) __attribute__((always_inline)) {       // base: the workgroup's row (uniform)
+        if (LINEAR) {
+            const char *pm = reinterpret_cast<const char *>(p.mean.p) + base * (int64_t)(AM * GL * sizeof(TM));
+            x.mu = *reinterpret_cast<const Pack<TM, AM> *>(pm + (uint32_t)(tid * AM * sizeof(TM)));
+            if (!SHARED) x.sd = *reinterpret_cast<const Pack<TM, AM> *>(reinterpret_cast<const char *>(p.log_std.p) + base * (int64_t)(AM * GL * sizeof(TM)) + (uint32_t)(tid * AM * sizeof(TM)));
+            const uint32_t o = (uint32_t)lane_row * 4u;
+            x.old = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.old.p) + base * 4 + o);
+            if (own_ref) x.ref = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.ref.p) + base * 4 + o);
+            x.adv = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.adv.p) + base * 4 + o);
+            if (masked) x.ok = maskp[base + (uint32_t)lane_row];
+        } else {
+#pragma unroll
+            for (int j = 0; j < AM; ++j)
+                if (j0 + j < p.A) {
+                    x.mu.v[j] = reinterpret_cast<const TM *>(p.mean.p)[o_mean + j * p.mean.sa];
+                    if (!SHARED) x.sd.v[j] = reinterpret_cast<const TM *>(p.log_std.p)[o_std + j * p.log_std.sa];
+                }
+            x.old = reinterpret_cast<const float *>(p.old.p)[o_old];
+            if (own_ref) x.ref = reinterpret_cast<const float *>(p.ref.p)[o_ref];
+            x.adv = reinterpret_cast<const float *>(p.adv.p)[o_adv];
+            if (masked) x.ok = maskp[o_mask];
         }
 #pragma unroll
-        for (int j = 0; j < AM; ++j) {
-            const bool has = PACKED || j0 + j < p.A;
-            if (!PACKED) {
-                mu[j] = has ? to_float(reinterpret_cast<const TM *>(p.mean.p)[o_mean + j * p.mean.sa]) : 0.f;
-                if (!SHARED) sd[j] = has ? to_float(reinterpret_cast<const TM *>(p.log_std.p)[o_std + j * p.log_std.sa]) : 0.f;
-            }
-            u[j] = has ? reinterpret_cast<const float *>(p.actions.p)[o_act + j * p.actions.sa] : 0.f;
+        for (int j = 0; j < AM; ++j)
+            if (LINEAR || j0 + j < p.A) x.u[j] = reinterpret_cast<const float *>(p.actions.p)[o_act + j * p.actions.sa];
+    };
+    auto move_on = [&]() __attribute__((always_inline)) {
+        i += di;
+        const bool nb = i >= p.n;
+        if (nb) i -= p.n;
+        auto move = [&](int64_t &o, const Rows &t) __attribute__((always_inline)) { o += db * t.sb + di * t.sn; if (nb) o += t.sb - p.n * t.sn; };
+        move(o_act, p.actions);
+        if (!LINEAR) {
+            move(o_mean, p.mean); move(o_old, p.old); move(o_adv, p.adv);
+            if (own_ref) move(o_ref, p.ref);
+            if (masked) move(o_mask, p.mask);
+            if (!SHARED) move(o_std, p.log_std);
         }
-        const double old = (double)reinterpret_cast<const float *>(p.old.p)[o_old];
-        const double ref = (double)reinterpret_cast<const float *>(p.ref.p)[o_ref];
-        const double adv = ((double)reinterpret_cast<const float *>(p.adv.p)[o_adv] - am) * ar;
-
-        double z[AM], e[AM], lp = 0.0, ent = 0.0;
+    };
+    Raw cur, nxt;
+    if (first + lane_row < last) fetch_row(cur, first);
+    for (int64_t base = first; base < last; base += ROWS) {
+        // (the GL lanes of a row go the same way)
+        const bool have = base + lane_row < last;
+        if (base + ROWS + lane_row < last) { move_on(); fetch_row(nxt, base + ROWS); }
+        const bool valid = have && (!masked || cur.ok != 0);
+        const double adv = ((double)cur.adv - am) * ar;
+        float zf[AM], ef[AM];
+        double lp = 0.0, ent = 0.0;
 #pragma unroll
         for (int j = 0; j < AM; ++j) {
-            if (PACKED || j0 + j < p.A) {
-                const double s = SHARED ? sh_s[j0 + j] : (double)sd[j];
-                e[j] = SHARED ? sh_e[j0 + j] : exp(-s);
-                z[j] = ((double)u[j] - (double)mu[j]) * e[j];
-                lp -= 0.5 * z[j] * z[j] + s + 0.91893853320467274178;   // log(2 pi) / 2
-                ent += s + 1.41893853320467274178;                      // (log(2 pi) + 1) / 2
+            if (LINEAR || j0 + j < p.A) {
+                const double s = SHARED ? sh_s[j0 + j] : (double)to_float(cur.sd.v[j]), e = SHARED ? sh_e[j0 + j] : exp(-s);
+                const double z = ((double)cur.u[j] - (double)to_float(cur.mu.v[j])) * e;
+                lp = __fma_rn(-0.5 * z, z, lp - (s + 0.91893853320467274178));        // log(2 pi) / 2
+                ent += s;
+                zf[j] = (float)z; ef[j] = (float)e;
             }
         }
 #pragma unroll
         for (int o = GL / 2; o; o >>= 1) { lp += __shfl_xor(lp, o, 64); ent += __shfl_xor(ent, o, 64); }
-        const double q = exp(lp - old), D = ref - lp, em = expm1(D);
-        const bool cut = (adv > 0.0 && q > p.hi) || (adv < 0.0 && q < p.lo);
-        const double g = valid ? w * ((cut ? 0.0 : -q * adv) - p.kl * em) : 0.0;
-        const double qa = q * adv, qc = (q < p.lo ? p.lo : q > p.hi ? p.hi : q) * adv;
+        const double d = lp - (double)cur.old;
+        double q, eD;
+        exp_both(d, q, eD);                                             // (without a reference of its own, D = -d)
+        float D = (float)-d, k3, em;
+        if (own_ref) {
+            const double Dd = (double)cur.ref - lp;
+            double unused;
+            exp_both(Dd, eD, unused);
+            D = (float)Dd;
+        }
+        expm1_parts(D, (float)eD, k3, em);
+        const bool above = d > p.dhi, below = d < p.dlo, cut = (adv > 0.0 && above) || (adv < 0.0 && below);
+        const double qa = q * adv;
+        const float g = w * ((cut ? 0.f : -(float)qa) - klf * em);
         if (valid && sub == 0) {
-            sum[0] += qa < qc ? qa : qc + (qa - qa);                     // min, and a NaN of either
-            sum[1] += em - D;
-            sum[2] += ent;
+            sum[0] += cut ? (above ? p.hi : p.lo) * adv : qa;            // min(q A, clip(q) A): the clipped one where it cuts
+            sum[1] += (double)k3;
+            sum[2] += ent + p.A * 1.41893853320467274178;               // (log(2 pi) + 1) / 2
             sum[3] += cut ? 1.0 : 0.0;
             sum[4] += q;
         }
@@ -156,32 +241,28 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
 #pragma unroll
         for (int j = 0; j < AM; ++j) {
             dm[j] = 0.f; ds[j] = 0.f;
-            if (PACKED || j0 + j < p.A) {
-                const double dsj = valid ? g * (z[j] * z[j] - 1.0) - p.ent * w : 0.0;
-                dm[j] = valid ? (float)(g * z[j] * e[j]) : 0.f;
-                if constexpr (SHARED) sum[LOSS_SUMS + j] += dsj;
-                else ds[j] = (float)dsj;
+            if ((LINEAR || j0 + j < p.A) && valid) {
+                dm[j] = g * zf[j] * ef[j];
+                ds[j] = __fmaf_rn(g, __fmaf_rn(zf[j], zf[j], -1.f), -entw);
+            }
+            if constexpr (SHARED) sum[LOSS_SUMS + j] += (double)ds[j];
+        }
+        if (have) {
+            if (LINEAR) {
+                char *pd = reinterpret_cast<char *>(p.dmean) + base * (int64_t)(AM * GL * sizeof(TM));
+                put<TM, AM>(pd, 0, (uint32_t)(tid * AM * sizeof(TM)), dm);
+                if (!SHARED) put<TM, AM>(reinterpret_cast<char *>(p.dstd) + base * (int64_t)(AM * GL * sizeof(TM)), 0, (uint32_t)(tid * AM * sizeof(TM)), ds);
+            } else {
+                const int64_t at = (base + lane_row) * p.A + j0;
+#pragma unroll
+                for (int j = 0; j < AM; ++j)
+                    if (j0 + j < p.A) {
+                        reinterpret_cast<TM *>(p.dmean)[at + j] = from_float<TM>(dm[j]);
+                        if (!SHARED) reinterpret_cast<TM *>(p.dstd)[at + j] = from_float<TM>(ds[j]);
+                    }
             }
         }
-        const int64_t at = r * p.A + j0;
-        if (PACKED) {
-            store_vec<TM, AM>(p.dmean, at, dm);
-            if (!SHARED) store_vec<TM, AM>(p.dstd, at, ds);
-        } else {
-#pragma unroll
-            for (int j = 0; j < AM; ++j)
-                if (j0 + j < p.A) {
-                    reinterpret_cast<TM *>(p.dmean)[at + j] = from_float<TM>(dm[j]);
-                    if (!SHARED) reinterpret_cast<TM *>(p.dstd)[at + j] = from_float<TM>(ds[j]);
-                }
-        }
-        i += di;
-        const bool nb = i >= p.n;
-        if (nb) i -= p.n;
-        auto move = [&](int64_t &o, const Rows &t) __attribute__((always_inline)) { o += db * t.sb + di * t.sn; if (nb) o += t.sb - p.n * t.sn; };
-        move(o_mean, p.mean); move(o_act, p.actions); move(o_old, p.old); move(o_ref, p.ref); move(o_adv, p.adv);
-        if (masked) move(o_mask, p.mask);
-        if (!SHARED) move(o_std, p.log_std);
+        cur = nxt;
     }
 #pragma unroll
     for (int k = 0; k < LOSS_SUMS; ++k) {
@@ -225,6 +306,7 @@ template <typename TM, bool SHARED> __global__ __launch_bounds__(512) void k_pol
     const int keys = LOSS_SUMS + (SHARED ? p.A : 0);
     for (int k = threadIdx.x >> 6; k < keys; k += 8) {
         double t = 0.0;
+#pragma unroll 8
         for (int g = threadIdx.x & 63; g < groups; g += 64) t += p.part[(int64_t)k * groups + g];
         t = wave_sum(t);
         if ((threadIdx.x & 63) == 0) tot[k] = t;

@@ -8,17 +8,19 @@
 //   memory, backward    G_t = dh_t + c_{t+1} (the gradient of h_t), c_t = a G_t, time reversed   A = a, S = a dh
 //                       dx = (1 - a) G, dgate = G (h_{t-1} - x_t) a (1 - a), dh0 = c_0
 //   advantages          delta = r + gamma (1 - done) V_{t+1} - V_t, time reversed          A = gamma lambda (1 - done), S = delta
-// A step at which the state is dropped (a reset, a finished episode) is A = -0.0: no product of the other coefficients,
-// which are never negative, has a sign, so the sign bit says "cut" through any composition and the state behind it is
-// selected away rather than multiplied by zero (it may be infinite or NaN).  A step beyond a sequence's length is the
-// identity (A = 1, S = 0).
+// Where the state is dropped (a reset, a finished episode), A = 0 and the state is selected away rather than multiplied by
+// it (it may be infinite or NaN).  The composition of a stretch that holds such a step has A = -0.0: coefficients are never
+// negative, so the sign says it.  A step beyond a sequence's length is the identity (A = 1, S = 0).
 //
 // Work split: a workgroup takes 64 V neighbouring channels (V a lane) and walks its stretch of time in tiles of NW x L
-// steps: wave w loads steps w L .. w L + L - 1 of the tile into registers, every load in flight at once, composes them,
-// leaves the pair in LDS, and behind one barrier composes the pairs of the waves in front of it and walks its own steps
-// again from registers.  Inputs are read once, outputs written once.  Where the channels alone do not fill the chip,
-// the time axis is cut into `nsplit` stretches: a first launch composes each stretch (its reads leave the data in the
-// last-level cache for the second), the second one starts each stretch from the composition of those before it.
+// steps: wave w has steps w L .. w L + L - 1 of the tile in registers, composes them, leaves the pair in LDS, and behind one
+// barrier composes the pairs of the waves in front of it and walks its own steps again from registers; the loads of its
+// next tile are in flight meanwhile.  Inputs are read once, outputs written once.  Where the channels alone do not fill
+// the chip, the time axis is cut into `nsplit` stretches: a first launch composes each stretch (its reads leave the data
+// in the last-level cache for the second), the second one starts each stretch from the composition of those before it.
+//
+// Addresses: a tensor's base at this step and at the workgroup's first sequence is uniform (scalar registers), a lane adds a
+// 32-bit byte offset (OFF = uint32_t), or a 64-bit one where a workgroup's sequences lie too far apart (OFF = int64_t).
 
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
 
@@ -36,24 +38,26 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(void *p, 
     *reinterpret_cast<Pack<T, V> *>(reinterpret_cast<T *>(p) + off) = r;
 }
 
-constexpr float CUT = -0.0f;
-__device__ __forceinline__ float apply(float A, float S, float y) { return (__float_as_uint(A) >> 31) ? S : __fmaf_rn(A, y, S); }
-
-// a = sigmoid(g), b = 1 - a, both to a few ulps at either end: the exponential of the negative magnitude never overflows
-// and the smaller of the two is e / (1 + e) itself.
+// a = sigmoid(g) and b = 1 - a from e = exp(-g): a = 1 / (1 + e), b = e a where e < 1 and 1 - a elsewhere, so neither end
+// loses digits and nothing is infinite times zero.  The exponential and the reciprocal are the hardware's (1 unit in the
+// last place each); what remains is the rounding of g log2(e), |g| units of e: with the sums, a and b are good to 4 + |g|
+// units.  (The correction of that rounding and a Newton step cost 9 of 22 instruction slots an element.)  NaN stays NaN.
 __device__ __forceinline__ void gate_pair(float g, float &a, float &b)
 {
-    const float e = expf(-fabsf(g)), p = 1.0f / (1.0f + e), q = e * p;
-    a = g >= 0.f ? p : q;
-    b = g >= 0.f ? q : p;
+    const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);
+    a = __builtin_amdgcn_rcpf(1.0f + e);
+    b = e < 1.0f ? e * a : 1.0f - a;
 }
 
 struct ScanGeom {
     int T, nsplit, Ts;              // steps, stretches, steps of a stretch (a multiple of the tile)
-    int64_t C;                      // channels
-    int64_t D;                      // channels of a sequence
-    float *ws;                      // [nsplit][2][C]: the composition of each stretch
+    uint32_t C;                     // channels
+    uint32_t D;                     // channels of a sequence
+    float *ws;                      // [nsplit][C][2]: the composition (A, S) of each stretch
 };
+
+// Where a lane is: its channel, its sequence's distance from the workgroup's first one and its place in the sequence.
+struct Place { uint32_t ch, b0, db, d; };
 
 // What cuts and ends the sequences of a memory (MSK: any of it given).
 struct Marks {
@@ -61,31 +65,77 @@ struct Marks {
     const uint8_t *resets;
     int64_t r_st, r_sb;
 };
-struct MarkLane { int len; int64_t r; };
-__device__ __forceinline__ MarkLane mark_lane(const Marks &m, int64_t b, int T)
+template <typename OFF> struct MarkLane { int len; OFF r; };
+template <typename OFF> __device__ __forceinline__ MarkLane<OFF> mark_lane(const Marks &m, const Place &w, int T)
 {
     int len = T;
-    if (m.lengths) { len = m.lengths[b]; len = len < 0 ? 0 : len > T ? T : len; }
-    return {len, b * m.r_sb};
+    if (m.lengths) { len = m.lengths[(size_t)w.b0 + w.db]; len = len < 0 ? 0 : len > T ? T : len; }
+    return {len, (OFF)((int64_t)w.db * m.r_sb)};
 }
 
-// ---- the operators: load() fetches step t of this lane's channels, coef() turns it into its map, step() applies it and
-// writes the step's outputs.  `on` is false beyond the stretch's end (the map is then the identity, nothing is written).
+template <typename T, typename S> __device__ __forceinline__ const char *base_of(const S &s, uint32_t b0) { return reinterpret_cast<const char *>(s.p) + (int64_t)b0 * s.sb * (int64_t)sizeof(T); }
+template <typename T, typename OFF, typename S> __device__ __forceinline__ OFF off_of(const S &s, const Place &w) { return (OFF)(((int64_t)w.db * s.sb + w.d) * (int64_t)sizeof(T)); }
+// V values as they lie in memory, in 32-bit words: a load in flight is not waited for by an unpacking the compiler moved
+// up to it.
+template <typename T, int V> struct Words;
+template <int V> struct Words<float, V> {
+    Pack<float, V> w;
+    __device__ __forceinline__ float get(int v) const { return w.v[v]; }
+    __device__ __forceinline__ void load(const char *p) { w = *reinterpret_cast<const Pack<float, V> *>(p); }
+};
+template <int V> struct Words<bf16, V> {
+    Pack<uint32_t, (V + 1) / 2> w;
+    __device__ __forceinline__ float get(int v) const { return __uint_as_float(v & 1 ? w.v[v / 2] & 0xffff0000u : w.v[v / 2] << 16); }
+    __device__ __forceinline__ void load(const char *p)
+    {
+        if constexpr (V == 1) w.v[0] = *reinterpret_cast<const uint16_t *>(p);
+        else w = *reinterpret_cast<const Pack<uint32_t, V / 2> *>(p);
+    }
+};
+template <int V> struct Words<uint8_t, V> {
+    uint32_t w;
+    __device__ __forceinline__ bool get(int v) const { return (w >> (8 * v)) & 0xffu; }
+    __device__ __forceinline__ void load(const char *p)
+    {
+        if constexpr (V == 1) w = *reinterpret_cast<const uint8_t *>(p);
+        else if constexpr (V == 2) w = *reinterpret_cast<const uint16_t *>(p);
+        else w = *reinterpret_cast<const uint32_t *>(p);
+    }
+};
+// A step is tb + dl with dl a constant of the unrolled loop: its offset is one product a tile and additions.
+struct Step { int tb, dl; __device__ __forceinline__ int t() const { return tb + dl; } };
+__device__ __forceinline__ int64_t step_off(const Step &s, int64_t st) { return (int64_t)s.tb * st + (int64_t)s.dl * st; }
+template <typename T, int V, typename OFF> __device__ __forceinline__ void fetch(Words<T, V> &o, const char *base, int64_t step, OFF off)
+{
+    o.load(base + step * (int64_t)sizeof(T) + off);
+}
+template <typename T, int V, typename OFF> __device__ __forceinline__ void put(const char *base, int64_t step, OFF off, const float (&x)[V])
+{
+    Pack<T, V> r;
+#pragma unroll
+    for (int v = 0; v < V; ++v) r.v[v] = from_float<T>(x[v]);
+    *reinterpret_cast<Pack<T, V> *>(const_cast<char *>(base) + step * (int64_t)sizeof(T) + off) = r;
+}
 
-template <typename T, int V, bool MSK> struct ForwardOp {
-    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false;
+// ---- the operators: fetch() loads step t of this lane's channels as it lies in memory, coef() turns it into its map, step()
+// applies it and writes the step's outputs.  `on` is false beyond the stretch's end (the map is then the identity, nothing
+// is written).
+
+template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
+    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false, CUTS = MSK;
     Seq gate, x;
     SeqOut out;
     const float *h0;
     float *h_last;
     Marks marks;
-    struct Lane { int64_t g, x, o; MarkLane m; };
-    struct Item { float A[V], S[V]; uint8_t cut; };
-    __device__ Lane lane(const ScanGeom &q, int64_t ch) const
+    struct Lane { const char *g, *x, *o, *r; OFF og, ox, oo; MarkLane<OFF> m; };
+    struct Raw { Words<T, V> g, x; Words<uint8_t, 1> cut; };
+    struct Item { float A[V], S[V]; bool cut; };
+    __device__ Lane lane(const ScanGeom &q, const Place &w) const
     {
-        const int64_t b = ch / q.D, d = ch - b * q.D;
-        Lane l{b * gate.sb + d, b * x.sb + d, b * out.sb + d, {}};
-        if (MSK) l.m = mark_lane(marks, b, q.T);
+        Lane l{base_of<T>(gate, w.b0), base_of<T>(x, w.b0), base_of<T>(out, w.b0), reinterpret_cast<const char *>(marks.resets) + (int64_t)w.b0 * marks.r_sb,
+               off_of<T, OFF>(gate, w), off_of<T, OFF>(x, w), off_of<T, OFF>(out, w), {}};
+        if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
     __device__ void carry0(float (&c)[V], int64_t ch) const
@@ -94,49 +144,55 @@ template <typename T, int V, bool MSK> struct ForwardOp {
         for (int v = 0; v < V; ++v) c[v] = 0.f;
         if (h0) load_vec<float, V>(c, h0, ch);
     }
-    __device__ void load(Item &i, const Lane &l, int t, bool) const
+    __device__ void load(Raw &i, const Lane &l, const Step &s, bool) const
     {
-        load_vec<T, V>(i.A, gate.p, l.g + (int64_t)t * gate.st);
-        load_vec<T, V>(i.S, x.p, l.x + (int64_t)t * x.st);
-        if (MSK) i.cut = marks.resets ? marks.resets[l.m.r + (int64_t)t * marks.r_st] : 0;
+        fetch(i.g, l.g, step_off(s, gate.st), l.og);
+        fetch(i.x, l.x, step_off(s, x.st), l.ox);
+        if (MSK) { i.cut.w = 0; if (marks.resets) fetch(i.cut, l.r, step_off(s, marks.r_st), l.m.r); }
     }
-    __device__ void coef(Item &i, const Lane &l, int t, bool on) const
+    __device__ void coef(Item &o, const Raw &i, const Lane &l, const Step &s, bool on) const
     {
-        if (MSK) on = on && t < l.m.len;
+        if (MSK) on = on && s.t() < l.m.len;
+        o.cut = MSK && on && i.cut.get(0);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float a, b;
-            gate_pair(i.A[v], a, b);
-            if (MSK && i.cut) a = CUT;
-            i.S[v] = on ? b * i.S[v] : 0.f;
-            i.A[v] = on ? a : 1.f;
+            gate_pair(i.g.get(v), a, b);
+            if (MSK && o.cut) a = 0.f;
+            o.S[v] = on ? b * i.x.get(v) : 0.f;
+            o.A[v] = on ? a : 1.f;
         }
     }
-    __device__ void step(float (&c)[V], const Item &i, const Lane &l, int t, bool on) const
+    __device__ void step(float (&c)[V], const Item &i, const Lane &l, const Step &s, bool on) const
     {
         float o[V];
-        const bool in = !MSK || t < l.m.len;
+        const bool in = !MSK || s.t() < l.m.len;
 #pragma unroll
-        for (int v = 0; v < V; ++v) { c[v] = apply(i.A[v], i.S[v], c[v]); o[v] = in ? c[v] : 0.f; }
-        if (on) store_vec<T, V>(out.p, l.o + (int64_t)t * out.st, o);
+        for (int v = 0; v < V; ++v) {
+            c[v] = __fmaf_rn(i.A[v], MSK && i.cut ? 0.f : c[v], i.S[v]);
+            o[v] = in ? c[v] : 0.f;
+        }
+        if (on) put<T, V>(l.o, step_off(s, out.st), l.oo, o);
     }
     __device__ void finish(const float (&c)[V], int64_t ch) const { if (h_last) store_vec<float, V>(h_last, ch, c); }
 };
 
-template <typename T, int V, bool MSK> struct BackwardOp {
-    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false;
+template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
+    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false, CUTS = MSK;
     Seq gate, x, h, dh;
     SeqOut dgate, dx;
     const float *h0, *dh_last;
     float *dh0;
     Marks marks;
-    struct Lane { int64_t g, x, h, dh, dg, dx, ch; MarkLane m; };
-    struct Item { float A[V], S[V], b[V], m[V], dh[V]; uint8_t cut; };
-    __device__ Lane lane(const ScanGeom &q, int64_t ch) const
+    struct Lane { const char *g, *x, *h, *dh, *dg, *dx, *r; OFF og, ox, oh, odh, odg, odx; uint32_t ch; MarkLane<OFF> m; };
+    struct Raw { Words<T, V> g, x, h, dh; Words<uint8_t, 1> cut; };
+    struct Item { float A[V], S[V], b[V], m[V], dh[V]; bool cut; };
+    __device__ Lane lane(const ScanGeom &q, const Place &w) const
     {
-        const int64_t b = ch / q.D, d = ch - b * q.D;
-        Lane l{b * gate.sb + d, b * x.sb + d, b * h.sb + d, b * dh.sb + d, b * dgate.sb + d, b * dx.sb + d, ch, {}};
-        if (MSK) l.m = mark_lane(marks, b, q.T);
+        Lane l{base_of<T>(gate, w.b0), base_of<T>(x, w.b0), base_of<T>(h, w.b0), base_of<T>(dh, w.b0), base_of<T>(dgate, w.b0), base_of<T>(dx, w.b0),
+               reinterpret_cast<const char *>(marks.resets) + (int64_t)w.b0 * marks.r_sb, off_of<T, OFF>(gate, w), off_of<T, OFF>(x, w), off_of<T, OFF>(h, w),
+               off_of<T, OFF>(dh, w), off_of<T, OFF>(dgate, w), off_of<T, OFF>(dx, w), w.ch, {}};
+        if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
     __device__ void carry0(float (&c)[V], int64_t ch) const
@@ -146,51 +202,55 @@ template <typename T, int V, bool MSK> struct BackwardOp {
         if (dh_last) load_vec<float, V>(c, dh_last, ch);
     }
     // agg: only what the composition needs
-    __device__ void load(Item &i, const Lane &l, int t, bool agg) const
+    __device__ void load(Raw &i, const Lane &l, const Step &s, bool agg) const
     {
-        load_vec<T, V>(i.A, gate.p, l.g + (int64_t)t * gate.st);
-        if (dh.p) load_vec<T, V>(i.dh, dh.p, l.dh + (int64_t)t * dh.st);
-        if (MSK) i.cut = marks.resets ? marks.resets[l.m.r + (int64_t)t * marks.r_st] : 0;
+        fetch(i.g, l.g, step_off(s, gate.st), l.og);
+        if (dh.p) fetch(i.dh, l.dh, step_off(s, dh.st), l.odh);
+        if (MSK) { i.cut.w = 0; if (marks.resets) fetch(i.cut, l.r, step_off(s, marks.r_st), l.m.r); }
         if (!agg) {
-            load_vec<T, V>(i.b, x.p, l.x + (int64_t)t * x.st);
-            load_vec<T, V>(i.m, h.p, l.h + (int64_t)(t > 0 ? t - 1 : 0) * h.st);
-            if (t == 0) {
-#pragma unroll
-                for (int v = 0; v < V; ++v) i.m[v] = 0.f;
-                if (h0) load_vec<float, V>(i.m, h0, l.ch);
-            }
+            fetch(i.x, l.x, step_off(s, x.st), l.ox);
+            fetch(i.h, l.h, s.t() > 0 ? step_off(Step{s.tb, s.dl - 1}, h.st) : 0, l.oh);
         }
     }
-    __device__ void coef(Item &i, const Lane &l, int t, bool on) const
+    __device__ void coef(Item &o, const Raw &i, const Lane &l, const Step &s, bool on) const
     {
-        if (MSK) on = on && t < l.m.len;
+        float before[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) before[v] = i.h.get(v);
+        if (s.t() == 0) {                                                    // (uniform)
+#pragma unroll
+            for (int v = 0; v < V; ++v) before[v] = 0.f;
+            if (h0) load_vec<float, V>(before, h0, l.ch);
+        }
+        if (MSK) on = on && s.t() < l.m.len;
+        o.cut = MSK && on && i.cut.get(0);
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             float a, b;
-            gate_pair(i.A[v], a, b);
-            const float dh_v = dh.p ? i.dh[v] : 0.f, before = (MSK && i.cut) ? 0.f : i.m[v];
-            i.m[v] = (before - i.b[v]) * a;                              // (h_{t-1} - x_t) a; x was loaded into b
-            i.b[v] = b;
-            i.dh[v] = dh_v;
-            i.S[v] = on ? a * dh_v : 0.f;
-            if (MSK && i.cut) { a = CUT; i.S[v] = 0.f; }
-            i.A[v] = on ? a : 1.f;
+            gate_pair(i.g.get(v), a, b);
+            const float d = dh.p ? i.dh.get(v) : 0.f;
+            o.m[v] = ((MSK && o.cut ? 0.f : before[v]) - i.x.get(v)) * a;       // (h_{t-1} - x_t) a
+            o.b[v] = b;
+            o.dh[v] = d;
+            if (MSK && o.cut) a = 0.f;
+            o.S[v] = on && !(MSK && o.cut) ? a * d : 0.f;
+            o.A[v] = on ? a : 1.f;
         }
     }
-    __device__ void step(float (&c)[V], const Item &i, const Lane &l, int t, bool on) const
+    __device__ void step(float (&c)[V], const Item &i, const Lane &l, const Step &s, bool on) const
     {
         float og[V], ox[V];
-        const bool in = !MSK || t < l.m.len;
+        const bool in = !MSK || s.t() < l.m.len;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
             const float G = (i.dh[v] + c[v]) * i.b[v];
             ox[v] = in ? G : 0.f;
             og[v] = in ? G * i.m[v] : 0.f;
-            c[v] = apply(i.A[v], i.S[v], c[v]);
+            c[v] = __fmaf_rn(i.A[v], MSK && i.cut ? 0.f : c[v], i.S[v]);
         }
         if (on) {
-            store_vec<T, V>(dgate.p, l.dg + (int64_t)t * dgate.st, og);
-            store_vec<T, V>(dx.p, l.dx + (int64_t)t * dx.st, ox);
+            put<T, V>(l.dg, step_off(s, dgate.st), l.odg, og);
+            put<T, V>(l.dx, step_off(s, dx.st), l.odx, ox);
         }
     }
     __device__ void finish(const float (&c)[V], int64_t ch) const { if (dh0) store_vec<float, V>(dh0, ch, c); }
@@ -198,7 +258,7 @@ template <typename T, int V, bool MSK> struct BackwardOp {
 
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.
 template <int V, bool MSK, bool MOM> struct AdvantageOp {
-    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM;
+    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK;
     const float *rewards, *values;
     int64_t rew_st, val_st, done_st;
     const uint8_t *dones;
@@ -206,16 +266,17 @@ template <int V, bool MSK, bool MOM> struct AdvantageOp {
     float gamma, lam;
     float *adv, *ret;
     int64_t C;
-    struct Lane { int64_t ch; int len[V]; };
-    struct Item { float A[V], S[V], val[V]; Pack<uint8_t, V> cut; };
-    __device__ Lane lane(const ScanGeom &q, int64_t ch) const
+    struct Lane { uint32_t ch; int len[V]; };
+    struct Raw { Words<float, V> r, v0, v1; Words<uint8_t, V> cut; };
+    struct Item { float A[V], S[V], val[V]; bool cut[V]; };
+    __device__ Lane lane(const ScanGeom &q, const Place &w) const
     {
-        Lane l{ch, {}};
+        Lane l{w.ch, {}};
         if (MSK) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 int n = q.T;
-                if (lengths) { n = lengths[(ch + v) / q.D]; n = n < 0 ? 0 : n > q.T ? q.T : n; }
+                if (lengths) { n = lengths[(w.ch + v) / q.D]; n = n < 0 ? 0 : n > q.T ? q.T : n; }
                 l.len[v] = n;
             }
         }
@@ -226,42 +287,51 @@ template <int V, bool MSK, bool MOM> struct AdvantageOp {
 #pragma unroll
         for (int v = 0; v < V; ++v) c[v] = 0.f;
     }
-    __device__ void load(Item &i, const Lane &l, int t, bool) const
+    static __device__ const char *at(const void *p) { return reinterpret_cast<const char *>(p); }
+    __device__ void load(Raw &i, const Lane &l, const Step &s, bool) const
     {
-        load_vec<float, V>(i.S, rewards, l.ch + (int64_t)t * rew_st);
-        load_vec<float, V>(i.val, values, l.ch + (int64_t)t * val_st);
-        load_vec<float, V>(i.A, values, l.ch + (int64_t)(t + 1) * val_st);
-        if (MSK && dones) i.cut = *reinterpret_cast<const Pack<uint8_t, V> *>(dones + l.ch + (int64_t)t * done_st);
+        fetch(i.r, at(rewards), step_off(s, rew_st), l.ch * 4u);
+        fetch(i.v0, at(values), step_off(s, val_st), l.ch * 4u);
+        fetch(i.v1, at(values), step_off(Step{s.tb, s.dl + 1}, val_st), l.ch * 4u);
+        if (MSK && dones) fetch(i.cut, at(dones), step_off(s, done_st), l.ch);
     }
-    __device__ void coef(Item &i, const Lane &l, int t, bool on) const
+    __device__ void coef(Item &o, const Raw &i, const Lane &l, const Step &s, bool on) const
     {
         const float gl = gamma * lam;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            const bool in = on && (!MSK || t < l.len[v]), cut = MSK && dones && i.cut.v[v];
-            const float delta = i.S[v] + (cut ? 0.f : gamma * i.A[v]) - i.val[v];
-            i.S[v] = in ? delta : 0.f;
-            i.A[v] = in ? (cut ? CUT : gl) : 1.f;
+            const bool in = on && (!MSK || s.t() < l.len[v]), cut = MSK && dones && i.cut.get(v);
+            const float delta = i.r.get(v) + (cut ? 0.f : gamma * i.v1.get(v)) - i.v0.get(v);
+            o.cut[v] = in && cut;
+            o.val[v] = i.v0.get(v);
+            o.S[v] = in ? delta : 0.f;
+            o.A[v] = in ? (cut ? 0.f : gl) : 1.f;
         }
     }
-    __device__ void step(float (&c)[V], const Item &i, const Lane &l, int t, bool on, double &s1, double &s2, int64_t &cnt) const
+    __device__ void step(float (&c)[V], const Item &i, const Lane &l, const Step &s, bool on, double &s1, double &s2, int &cnt) const
     {
         float oa[V], ov[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-            c[v] = apply(i.A[v], i.S[v], c[v]);
-            const bool in = on && (!MSK || t < l.len[v]);
+            c[v] = __fmaf_rn(i.A[v], MSK && i.cut[v] ? 0.f : c[v], i.S[v]);
+            const bool in = on && (!MSK || s.t() < l.len[v]);
             oa[v] = in ? c[v] : 0.f;
             ov[v] = in ? c[v] + i.val[v] : 0.f;
             if (MOM && in) { s1 += (double)c[v]; s2 += (double)c[v] * (double)c[v]; ++cnt; }
         }
         if (on) {
-            store_vec<float, V>(adv, l.ch + (int64_t)t * C, oa);
-            store_vec<float, V>(ret, l.ch + (int64_t)t * C, ov);
+            put<float, V>(at(adv), step_off(s, C), l.ch * 4u, oa);
+            put<float, V>(at(ret), step_off(s, C), l.ch * 4u, ov);
         }
     }
     __device__ void finish(const float (&)[V], int64_t) const {}
 };
+
+template <class Item> __device__ __forceinline__ bool cut_of(const Item &i, int v)
+{
+    if constexpr (std::is_array_v<decltype(i.cut)>) return i.cut[v];
+    else return i.cut;
+}
 
 // Moments of the advantages: a partial (count, sum, sum of squares) per workgroup in double, summed in a fixed order.
 __device__ __forceinline__ double wave_sum(double x)
@@ -271,102 +341,162 @@ __device__ __forceinline__ double wave_sum(double x)
     return x;
 }
 
+// y behind a stretch whose composition is (A, S)
+template <bool CUTS> __device__ __forceinline__ float through(float A, float S, float y)
+{
+    const float r = __fmaf_rn(A, y, S);
+    return CUTS && (__float_as_uint(A) >> 31) ? S : r;
+}
+template <bool CUTS> __device__ __forceinline__ float joined(float A, float A0) { return CUTS && (__float_as_uint(A) >> 31) ? -0.f : A * A0; }
+
 // V channels a lane, NW waves, L steps a wave and tile.  AGG: the stretch's composition only.
 template <class Op, int V, int NW, int L, bool AGG>
 __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom)
 {
-    __shared__ alignas(16) float ex[2][NW][2][64][V];
+    constexpr bool CUTS = Op::CUTS;
+    __shared__ alignas(16) float ex[NW > 1 ? 2 : 1][NW][2][64][V];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), split = blockIdx.y;
-    const int64_t ch0 = ((int64_t)blockIdx.x * 64 + lane) * V;
-    const bool have = ch0 < q.C;
-    const int64_t ch = have ? ch0 : 0;                                  // (lanes beyond the channels read channel 0 and write nothing)
-    const typename Op::Lane ln = op.lane(q, ch);
+    const uint32_t first = blockIdx.x * 64u * V, mine_ch = first + lane * V;
+    const bool have = mine_ch < q.C;
+    Place w;
+    w.ch = have ? mine_ch : first;                                      // (lanes beyond the channels read the workgroup's first one and write nothing)
+    w.b0 = __builtin_amdgcn_readfirstlane(first / q.D);
+    const uint32_t rel = w.ch - w.b0 * q.D;
+    w.db = rel / q.D;
+    w.d = rel - w.db * q.D;
+    const typename Op::Lane ln = op.lane(q, w);
     const int lo = split * q.Ts, hi = lo + q.Ts < q.T ? lo + q.Ts : q.T;
+    typename Op::Raw raw[L];
+    auto step_at = [&](int u0, int l) __attribute__((always_inline)) { return Op::REVERSE ? Step{q.T - 1 - u0, -l} : Step{u0, l}; };
+    // CLAMP: a step beyond the end reads the last one again, and is not used
+    auto load_tile = [&](auto clamp, int tile) __attribute__((always_inline)) {
+        const int u0 = tile + wave * L;
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            if (decltype(clamp)::value) op.load(raw[l], ln, step_at(u0 + l < hi ? u0 + l : hi - 1, 0), AGG);
+            else op.load(raw[l], ln, step_at(u0, l), AGG);
+        }
+    };
+    if (lo < hi) load_tile(std::true_type{}, lo);
     float CA[V], c[V];                                                  // AGG: (CA, c) is the composition so far; else c is the state
     if (AGG) {
 #pragma unroll
         for (int v = 0; v < V; ++v) { CA[v] = 1.f; c[v] = 0.f; }
     } else {
-        op.carry0(c, ch);
-        for (int j = 0; j < split; ++j) {
-            float A[V], S[V];
-            load_vec<float, V>(A, q.ws, (int64_t)(2 * j) * q.C + ch);
-            load_vec<float, V>(S, q.ws, (int64_t)(2 * j + 1) * q.C + ch);
+        op.carry0(c, w.ch);
+        if (split > 0) {                                                // the stretches before this one, a part of them by each wave
+            float PA[V], PS[V];
 #pragma unroll
-            for (int v = 0; v < V; ++v) c[v] = apply(A[v], S[v], c[v]);
+            for (int v = 0; v < V; ++v) { PA[v] = 1.f; PS[v] = 0.f; }
+            const int j1 = (wave + 1) * split / NW;
+            int j = wave * split / NW;
+            auto join = [&](const float (&m)[2 * V]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) { PS[v] = through<CUTS>(m[2 * v], m[2 * v + 1], PS[v]); PA[v] = joined<CUTS>(m[2 * v], PA[v]); }
+            };
+            for (; j + 16 <= j1; j += 16) {                             // (sixteen loads in flight: another XCD wrote them, they come from memory)
+                float m[16][2 * V];
+#pragma unroll
+                for (int k = 0; k < 16; ++k) load_vec<float, 2 * V>(m[k], q.ws, ((int64_t)(j + k) * q.C + w.ch) * 2);
+#pragma unroll
+                for (int k = 0; k < 16; ++k) join(m[k]);
+            }
+            float m[16][2 * V];
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (j + k < j1) load_vec<float, 2 * V>(m[k], q.ws, ((int64_t)(j + k) * q.C + w.ch) * 2);
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+                if (j + k < j1) join(m[k]);
+#pragma unroll
+            for (int v = 0; v < V; ++v) { ex[0][wave][0][lane][v] = PA[v]; ex[0][wave][1][lane][v] = PS[v]; }
+            __syncthreads();
+#pragma unroll
+            for (int k = 0; k < NW; ++k)
+#pragma unroll
+                for (int v = 0; v < V; ++v) c[v] = through<CUTS>(ex[0][k][0][lane][v], ex[0][k][1][lane][v], c[v]);
         }
     }
     double s1 = 0, s2 = 0;
-    int64_t cnt = 0;
-    int par = 0;
-    for (int tile = lo; tile < hi; tile += NW * L) {
+    int cnt = 0;
+    int par = 1;                                                        // (the half the stretches were not left in)
+    // FULL: every step of the tile lies inside the stretch.  NEXT: the next tile is 0 none, 1 perhaps partly beyond the end, 2 full.
+    auto work = [&](auto full, auto next, int tile) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value;
+        constexpr int NEXT = decltype(next)::value;
         const int u0 = tile + wave * L;
         typename Op::Item it[L];
+        float PA[V], PS[V], mine[V];                                    // mine: the state in front of this wave's steps
+        bool any[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) { PA[v] = 1.f; PS[v] = 0.f; any[v] = false; mine[v] = c[v]; }
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-            const int u = u0 + l < hi ? u0 + l : hi - 1;                // (steps beyond the end: the last one again, not used)
-            op.load(it[l], ln, Op::REVERSE ? q.T - 1 - u : u, AGG);
-        }
-        float PA[V], PS[V];
+            op.coef(it[l], raw[l], ln, step_at(u0, l), FULL || u0 + l < hi);
+            if (NW > 1 || AGG) {
 #pragma unroll
-        for (int v = 0; v < V; ++v) { PA[v] = 1.f; PS[v] = 0.f; }
-#pragma unroll
-        for (int l = 0; l < L; ++l) {
-            const int u = u0 + l;
-            op.coef(it[l], ln, Op::REVERSE ? q.T - 1 - u : u, u < hi);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                PS[v] = apply(it[l].A[v], it[l].S[v], PS[v]);
-                PA[v] = (__float_as_uint(it[l].A[v]) >> 31) ? CUT : it[l].A[v] * PA[v];
+                for (int v = 0; v < V; ++v) {
+                    const bool cut = CUTS && cut_of(it[l], v);
+                    PS[v] = __fmaf_rn(it[l].A[v], cut ? 0.f : PS[v], it[l].S[v]);
+                    PA[v] *= it[l].A[v];
+                    any[v] = any[v] || cut;
+                }
             }
         }
-        float mine[V];                                                  // the state in front of this wave's steps
-        if (NW > 1) {
+        if constexpr (NEXT != 0) load_tile(std::bool_constant<NEXT == 1>{}, tile + NW * L);
+        if constexpr (NW > 1) {
 #pragma unroll
-            for (int v = 0; v < V; ++v) { ex[par][wave][0][lane][v] = PA[v]; ex[par][wave][1][lane][v] = PS[v]; }
+            for (int v = 0; v < V; ++v) { ex[par][wave][0][lane][v] = CUTS && any[v] ? -0.f : PA[v]; ex[par][wave][1][lane][v] = PS[v]; }
             __syncthreads();
 #pragma unroll
-            for (int w = 0; w < NW; ++w) {
-                if (w == wave) {
+            for (int k = 0; k < NW; ++k) {
+                if (k == wave) {
 #pragma unroll
                     for (int v = 0; v < V; ++v) mine[v] = c[v];
                 }
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    const float A = ex[par][w][0][lane][v], S = ex[par][w][1][lane][v];
-                    c[v] = apply(A, S, c[v]);
-                    if (AGG) CA[v] = (__float_as_uint(A) >> 31) ? CUT : A * CA[v];
+                    const float A = ex[par][k][0][lane][v], S = ex[par][k][1][lane][v];
+                    c[v] = through<CUTS>(A, S, c[v]);
+                    if (AGG) CA[v] = joined<CUTS>(A, CA[v]);
                 }
             }
             par ^= 1;                                                   // (the next tile's pairs go to the other half: one barrier a tile)
-        } else {
+        } else if (AGG) {
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                mine[v] = c[v];
-                if (AGG) { c[v] = apply(PA[v], PS[v], c[v]); CA[v] = (__float_as_uint(PA[v]) >> 31) ? CUT : PA[v] * CA[v]; }
+                const float A = CUTS && any[v] ? -0.f : PA[v];
+                c[v] = through<CUTS>(A, PS[v], c[v]);
+                CA[v] = joined<CUTS>(A, CA[v]);
             }
         }
         if (!AGG) {
 #pragma unroll
             for (int l = 0; l < L; ++l) {
-                const int u = u0 + l, t = Op::REVERSE ? q.T - 1 - u : u;
-                if constexpr (Op::SUMS) op.step(mine, it[l], ln, t, have && u < hi, s1, s2, cnt);
-                else op.step(mine, it[l], ln, t, have && u < hi);
+                const bool on = have && (FULL || u0 + l < hi);
+                if constexpr (Op::SUMS) op.step(mine, it[l], ln, step_at(u0, l), on, s1, s2, cnt);
+                else op.step(mine, it[l], ln, step_at(u0, l), on);
             }
             if (NW == 1) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) c[v] = mine[v];
             }
         }
-    }
+    };
+    int tile = lo;
+    for (; tile + 2 * NW * L <= hi; tile += NW * L) work(std::true_type{}, std::integral_constant<int, 2>{}, tile);
+    if (tile + NW * L < hi) { work(std::true_type{}, std::integral_constant<int, 1>{}, tile); tile += NW * L; }
+    if (tile < hi) work(std::false_type{}, std::integral_constant<int, 0>{}, tile);
     if (AGG) {
         if (have && wave == 0) {
-            store_vec<float, V>(q.ws, (int64_t)(2 * split) * q.C + ch, CA);
-            store_vec<float, V>(q.ws, (int64_t)(2 * split + 1) * q.C + ch, c);
+            float m[2 * V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) { m[2 * v] = CA[v]; m[2 * v + 1] = c[v]; }
+            store_vec<float, 2 * V>(q.ws, ((int64_t)split * q.C + w.ch) * 2, m);
         }
         return;
     }
-    if (have && wave == 0 && split == q.nsplit - 1) op.finish(c, ch);
+    if (have && wave == 0 && split == q.nsplit - 1) op.finish(c, w.ch);
     if constexpr (Op::MOMENTS) {
         __shared__ double red[NW][3];
         const double w1 = wave_sum(s1), w2 = wave_sum(s2), w0 = wave_sum((double)cnt);
@@ -374,7 +504,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
         __syncthreads();
         if (threadIdx.x < 3) {
             double t = 0;
-            for (int w = 0; w < NW; ++w) t += red[w][threadIdx.x];
+            for (int k = 0; k < NW; ++k) t += red[k][threadIdx.x];
             mom[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 3 + threadIdx.x] = t;
         }
     }
@@ -420,7 +550,7 @@ __global__ __launch_bounds__(256) void k_scan_step(int64_t n, int64_t D, const v
     for (int v = 0; v < V; ++v) {
         float a, k;
         gate_pair(g[v], a, k);
-        s[v] = apply(cut ? CUT : a, k * xv[v], s[v]);
+        s[v] = __fmaf_rn(cut ? 0.f : a, cut ? 0.f : s[v], k * xv[v]);
     }
     store_vec<float, V>(state, e, s);
     store_vec<T, V>(out, b * o_sb + d, s);

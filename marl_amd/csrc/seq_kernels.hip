@@ -4,6 +4,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 #include <algorithm>
+#include <cmath>
+#include <initializer_list>
+#include <type_traits>
 
 #include "seq_kernels.h"
 
@@ -24,72 +27,99 @@ namespace {
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 bool vec_ok(const void *p, int64_t st, int64_t sb, size_t elem, int V) { return !p || (aligned(p, elem * V) && st % V == 0 && sb % V == 0); }
 
-struct Plan { int V, nsplit, Ts; };
+// How a scan is laid out: V channels a lane, NW waves that share a tile of time, L steps a wave and tile; nsplit stretches of Ts steps.
+struct Plan { int V, NW, L, nsplit, Ts; };
 
-constexpr int NW = 4, LF = 8, LB = 4;
-
-// Channels a lane takes and stretches of the time axis.
-Plan scan_plan(int64_t T, int64_t C, bool vec)
+// By C, the channels, and `size`, the bytes of a value (forward + backward of 200 steps, float32 / bfloat16, us):
+//   C       1 channel a lane, 4 waves a tile   2 channels, 4 waves   4 channels, one wave walks all of time
+//   30720              39 / 32                      41 / 32                     110 / 114
+//   62848              77 / 49                      75 / 42                     128 / 114
+//   122880            179 / 97                     164 / 80                     172 / 145
+//   245760            361 / 205                    359 / 176                    312 / 182
+//   491520            706 / 401                    695 / 359                    676 / 325
+// Many channels fill the chip by themselves, and a wave that shares nothing waits for nobody: from 600 KB a time step on.  Below,
+// four waves side by side in time; from 49152 channels on two of them in a lane (half the address work).  Rows that are not aligned to two or four
+// values go one channel a lane.  Fewer than 256 workgroups and ten tiles of time or more: the time axis is cut until there are 512,
+// down to one tile a stretch (20011 steps x 183 channels, forward + backward: 61 stretches 97 us, 157 stretches 61 us; 1920 channels
+// forward, cut / whole: 256 steps 7.8 / 8.4 us, 192 steps 7.7 / 7.1 us, and a launch less on the host).
+Plan scan_plan(int64_t T, int64_t C, size_t size, bool vec2, bool vec4)
 {
-    Plan p{vec && C >= 65536 ? 4 : 1, 1, 0};
-    const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V), tile = NW * LF;
-    int64_t want = groups >= 256 ? 1 : 512 / groups;
-    want = std::min<int64_t>(want, T / (4 * tile));
-    want = std::max<int64_t>(1, std::min<int64_t>(want, 64));
-    const int64_t tiles = (T + tile - 1) / tile, per = (tiles + want - 1) / want;
-    p.Ts = (int)(std::max<int64_t>(per, 1) * tile);
-    p.nsplit = (int)std::max<int64_t>(1, (T + p.Ts - 1) / p.Ts);
+    Plan p{1, 4, 8, 1, 0};
+    if (vec4 && C * (int64_t)size >= 600000) p = {4, 1, 4, 1, 0};
+    else if (vec2 && C >= 49152) p = {2, 4, 4, 1, 0};
+    const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V), tile = p.NW * p.L, tiles = std::max<int64_t>(1, (T + tile - 1) / tile);
+    int64_t want = 1;
+    if (p.V == 1 && groups < 256 && tiles >= 10) want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / groups, tiles), 256));
+    const int64_t per = (tiles + want - 1) / want;
+    p.Ts = (int)(per * tile);
+    p.nsplit = (int)((tiles + per - 1) / per);
     return p;
 }
+// (the workspace of any alignment)
+int most_splits(int64_t T, int64_t C, size_t size) { return scan_plan(T, C, size, false, false).nsplit; }
 
-template <template <typename, int, bool> class Op, typename T, int V, bool MSK, int L, class Fill>
-int scan_go(const ScanGeom &q, Fill fill, hipStream_t st)
+template <int V, int NW, int L, class O> int scan_go(const O &op, const ScanGeom &q, double *mom, hipStream_t st)
 {
-    Op<T, V, MSK> op;
-    fill(op);
     const unsigned groups = (unsigned)((q.C + 64 * V - 1) / (64 * V));
-    if (q.nsplit > 1) {
-        hipLaunchKernelGGL((k_scan<Op<T, V, MSK>, V, NW, L, true>), dim3(groups, q.nsplit - 1), dim3(64 * NW), 0, st, op, q, (double *)nullptr);
-        LAUNCH_CHECK();
-    }
-    hipLaunchKernelGGL((k_scan<Op<T, V, MSK>, V, NW, L, false>), dim3(groups, q.nsplit), dim3(64 * NW), 0, st, op, q, (double *)nullptr);
+    if constexpr (V == 1)
+        if (q.nsplit > 1) {
+            hipLaunchKernelGGL((k_scan<O, V, NW, L, true>), dim3(groups, q.nsplit - 1), dim3(64 * NW), 0, st, op, q, (double *)nullptr);
+            LAUNCH_CHECK();
+        }
+    hipLaunchKernelGGL((k_scan<O, V, NW, L, false>), dim3(groups, q.nsplit), dim3(64 * NW), 0, st, op, q, mom);
     LAUNCH_CHECK();
     return 0;
 }
-template <template <typename, int, bool> class Op, int L, class Fill>
-int scan_dispatch(int dtype, int V, bool msk, const ScanGeom &q, Fill fill, hipStream_t st)
+template <template <typename, int, bool, typename> class Op, typename T, bool MSK, class Fill>
+int scan_typed(const Plan &p, bool far, const ScanGeom &q, Fill fill, hipStream_t st)
 {
-#define GO(T, VV) (msk ? scan_go<Op, T, VV, true, L>(q, fill, st) : scan_go<Op, T, VV, false, L>(q, fill, st))
-    if (dtype == 0) return V == 4 ? GO(float, 4) : GO(float, 1);
-    return V == 4 ? GO(bf16, 4) : GO(bf16, 1);
-#undef GO
+    if (p.V == 4) { Op<T, 4, MSK, uint32_t> op; fill(op); return scan_go<4, 1, 4>(op, q, nullptr, st); }
+    if (p.V == 2) { Op<T, 2, MSK, uint32_t> op; fill(op); return scan_go<2, 4, 4>(op, q, nullptr, st); }
+    if (far) { Op<T, 1, MSK, int64_t> op; fill(op); return scan_go<1, 4, 8>(op, q, nullptr, st); }
+    Op<T, 1, MSK, uint32_t> op;
+    fill(op);
+    return scan_go<1, 4, 8>(op, q, nullptr, st);
+}
+template <template <typename, int, bool, typename> class Op, class Fill>
+int scan_dispatch(int dtype, bool msk, const Plan &p, bool far, const ScanGeom &q, Fill fill, hipStream_t st)
+{
+    if (dtype == 0) return msk ? scan_typed<Op, float, true>(p, far, q, fill, st) : scan_typed<Op, float, false>(p, far, q, fill, st);
+    return msk ? scan_typed<Op, bf16, true>(p, far, q, fill, st) : scan_typed<Op, bf16, false>(p, far, q, fill, st);
+}
+
+// Whether a workgroup's sequences lie too far apart for 32-bit byte offsets (V: the most channels a lane may take).
+bool too_far(int64_t D, std::initializer_list<int64_t> strides, size_t elem)
+{
+    int64_t sb = 0;
+    for (int64_t s : strides) sb = std::max(sb, s);
+    const int64_t rows = 64 * 4 / D + 2;
+    return (double)rows * (double)sb * (double)elem + (double)D * (double)elem >= 4294967296.0;
 }
 
 }  // namespace
 
-int64_t scan_workspace(int, int64_t T, int64_t B, int64_t D)
+int64_t scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
 {
-    const int64_t C = B * D;                                            // (the larger of the two plans)
-    const int n = std::max(scan_plan(T, C, true).nsplit, scan_plan(T, C, false).nsplit);
-    return n > 1 ? (int64_t)n * 2 * C * 4 : 0;
+    const int n = most_splits(T, B * D, dtype ? 2 : 4);
+    return n > 1 ? (int64_t)n * 2 * B * D * 4 : 0;
 }
 
-static ScanGeom scan_geom(const ScanArgs &a, bool vec, int *V)
+static ScanGeom scan_geom(const ScanArgs &a, const Plan &p)
 {
-    const Plan p = scan_plan(a.T, a.B * a.D, vec);
-    *V = p.V;
-    return {(int)a.T, p.nsplit, p.Ts, a.B * a.D, a.D, reinterpret_cast<float *>(a.ws)};
+    return {(int)a.T, p.nsplit, p.Ts, (uint32_t)(a.B * a.D), (uint32_t)a.D, reinterpret_cast<float *>(a.ws)};
 }
 
 int launch_scan_forward(const ScanArgs &a, hipStream_t st)
 {
     if (a.B * a.D == 0) return 0;
     const size_t e = a.dtype ? 2 : 4;
-    const bool vec = a.D % 4 == 0 && vec_ok(a.gate.p, a.gate.st, a.gate.sb, e, 4) && vec_ok(a.x.p, a.x.st, a.x.sb, e, 4) &&
-                     vec_ok(a.out.p, a.out.st, a.out.sb, e, 4) && aligned(a.h0, 16) && aligned(a.h_last, 16) && aligned(a.ws, 16);
-    int V;
-    const ScanGeom q = scan_geom(a, vec, &V);
-    return scan_dispatch<ForwardOp, LF>(a.dtype, V, a.resets || a.lengths, q, [&](auto &op) {
+    const bool far = too_far(a.D, {a.gate.sb, a.x.sb, a.out.sb, a.r_sb}, e);
+    const auto rows = [&](int V) {
+        return !far && a.D % V == 0 && vec_ok(a.gate.p, a.gate.st, a.gate.sb, e, V) && vec_ok(a.x.p, a.x.st, a.x.sb, e, V) &&
+               vec_ok(a.out.p, a.out.st, a.out.sb, e, V) && aligned(a.h0, 4 * V) && aligned(a.h_last, 4 * V);
+    };
+    const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
+    return scan_dispatch<ForwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
         op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last;
         op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
     }, st);
@@ -99,12 +129,14 @@ int launch_scan_backward(const ScanArgs &a, hipStream_t st)
 {
     if (a.B * a.D == 0) return 0;
     const size_t e = a.dtype ? 2 : 4;
-    const bool vec = a.D % 4 == 0 && vec_ok(a.gate.p, a.gate.st, a.gate.sb, e, 4) && vec_ok(a.x.p, a.x.st, a.x.sb, e, 4) &&
-                     vec_ok(a.h.p, a.h.st, a.h.sb, e, 4) && vec_ok(a.dh.p, a.dh.st, a.dh.sb, e, 4) && vec_ok(a.dgate.p, a.dgate.st, a.dgate.sb, e, 4) &&
-                     vec_ok(a.dx.p, a.dx.st, a.dx.sb, e, 4) && aligned(a.h0, 16) && aligned(a.dh_last, 16) && aligned(a.dh0, 16) && aligned(a.ws, 16);
-    int V;
-    const ScanGeom q = scan_geom(a, vec, &V);
-    return scan_dispatch<BackwardOp, LB>(a.dtype, V, a.resets || a.lengths, q, [&](auto &op) {
+    const bool far = too_far(a.D, {a.gate.sb, a.x.sb, a.h.sb, a.dh.sb, a.dgate.sb, a.dx.sb, a.r_sb}, e);
+    const auto rows = [&](int V) {
+        return !far && a.D % V == 0 && vec_ok(a.gate.p, a.gate.st, a.gate.sb, e, V) && vec_ok(a.x.p, a.x.st, a.x.sb, e, V) && vec_ok(a.h.p, a.h.st, a.h.sb, e, V) &&
+               vec_ok(a.dh.p, a.dh.st, a.dh.sb, e, V) && vec_ok(a.dgate.p, a.dgate.st, a.dgate.sb, e, V) && vec_ok(a.dx.p, a.dx.st, a.dx.sb, e, V) &&
+               aligned(a.h0, 4 * V) && aligned(a.dh_last, 4 * V) && aligned(a.dh0, 4 * V);
+    };
+    const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
+    return scan_dispatch<BackwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
         op.gate = a.gate; op.x = a.x; op.h = a.h; op.dh = a.dh; op.dgate = a.dgate; op.dx = a.dx;
         op.h0 = a.h0; op.dh_last = a.dh_last; op.dh0 = a.dh0;
         op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
@@ -127,33 +159,22 @@ int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t 
     return 0;
 }
 
-// [nsplit][2][C] floats, then three doubles a workgroup
+// The stretches' compositions, then three doubles a workgroup.
 int64_t advantages_workspace(int64_t T, int64_t C)
 {
-    int64_t most = 0;
-    for (int v = 0; v < 2; ++v) {
-        const Plan p = scan_plan(T, C, v);
-        const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V);
-        most = std::max(most, (p.nsplit > 1 ? (int64_t)p.nsplit * 2 * C * 4 + 16 : 0) + groups * p.nsplit * 24);
-    }
-    return most;
+    const int n = most_splits(T, C, 4);
+    return (n > 1 ? (int64_t)n * 2 * C * 4 + 16 : 0) + (C + 63) / 64 * n * 24;
 }
 
-template <int V, bool MSK, bool MOM> static int advantages_go(const AdvArgs &a, const Plan &p, hipStream_t st)
+template <int V, int NW, int L, bool MSK, bool MOM> static int advantages_go(const AdvArgs &a, const Plan &p, hipStream_t st)
 {
     AdvantageOp<V, MSK, MOM> op;
     op.rewards = a.rewards; op.values = a.values; op.rew_st = a.rew_st; op.val_st = a.val_st; op.done_st = a.done_st;
     op.dones = a.dones; op.lengths = a.lengths; op.gamma = a.gamma; op.lam = a.lam; op.adv = a.adv; op.ret = a.ret; op.C = a.C;
     const unsigned groups = (unsigned)((a.C + 64 * V - 1) / (64 * V));
-    ScanGeom q{(int)a.T, p.nsplit, p.Ts, a.C, a.D, reinterpret_cast<float *>(a.ws)};
+    ScanGeom q{(int)a.T, p.nsplit, p.Ts, (uint32_t)a.C, (uint32_t)a.D, reinterpret_cast<float *>(a.ws)};
     double *mom = reinterpret_cast<double *>(reinterpret_cast<char *>(a.ws) + (p.nsplit > 1 ? ((int64_t)p.nsplit * 2 * a.C * 4 + 15) / 16 * 16 : 0));
-    if (p.nsplit > 1) {
-        hipLaunchKernelGGL((k_scan<AdvantageOp<V, MSK, MOM>, V, NW, LF, true>), dim3(groups, p.nsplit - 1), dim3(64 * NW), 0, st, op, q,
-                           (double *)nullptr);
-        LAUNCH_CHECK();
-    }
-    hipLaunchKernelGGL((k_scan<AdvantageOp<V, MSK, MOM>, V, NW, LF, false>), dim3(groups, p.nsplit), dim3(64 * NW), 0, st, op, q, mom);
-    LAUNCH_CHECK();
+    if (int rc = scan_go<V, NW, L>(op, q, mom, st)) return rc;
     if (MOM) {
         hipLaunchKernelGGL(k_moments, dim3(1), dim3(256), 0, st, mom, (int64_t)groups * p.nsplit, a.moments);
         LAUNCH_CHECK();
@@ -163,18 +184,21 @@ template <int V, bool MSK, bool MOM> static int advantages_go(const AdvArgs &a, 
 
 int launch_advantages(const AdvArgs &a, hipStream_t st)
 {
-    const bool vec = a.C % 4 == 0 && vec_ok(a.rewards, a.rew_st, 0, 4, 4) && vec_ok(a.values, a.val_st, 0, 4, 4) &&
-                     vec_ok(a.dones, a.done_st, 0, 1, 4) && aligned(a.adv, 16) && aligned(a.ret, 16) && aligned(a.ws, 16);
-    const Plan p = scan_plan(a.T, a.C, vec);
+    const auto rows = [&](int V) {
+        return a.C % V == 0 && vec_ok(a.rewards, a.rew_st, 0, 4, V) && vec_ok(a.values, a.val_st, 0, 4, V) && vec_ok(a.dones, a.done_st, 0, 1, V) &&
+               aligned(a.adv, 4 * V) && aligned(a.ret, 4 * V);
+    };
+    Plan p = scan_plan(a.T, a.C, 4, false, false);
+    if (rows(4) && a.C >= 49152) p = {4, 4, 4, 1, (int)((a.T + 15) / 16 * 16)};        // (200 x 122880: 75 us; two channels a lane 80 us, one wave for all of time 82 us)
     const bool msk = a.dones || a.lengths, mom = a.moments != nullptr;
-#define GO(V, M) (mom ? advantages_go<V, M, true>(a, p, st) : advantages_go<V, M, false>(a, p, st))
-    if (p.V == 4) return msk ? GO(4, true) : GO(4, false);
-    return msk ? GO(1, true) : GO(1, false);
+#define GO(V, NW, L) (msk ? (mom ? advantages_go<V, NW, L, true, true>(a, p, st) : advantages_go<V, NW, L, true, false>(a, p, st)) \
+                          : (mom ? advantages_go<V, NW, L, false, true>(a, p, st) : advantages_go<V, NW, L, false, false>(a, p, st)))
+    return p.V == 4 ? GO(4, 4, 4) : GO(1, 4, 8);
 #undef GO
 }
 
 namespace {
-constexpr int LOSS_GROUPS = 2048, COUNT_GROUPS = 512;
+constexpr int LOSS_GROUPS = 1024, COUNT_GROUPS = 512;
 int lanes_of(int A) { return A <= 4 ? 1 : A <= 8 ? 2 : A <= 16 ? 4 : 8; }
 int loss_groups(int64_t rows, int A) { return (int)std::min<int64_t>((rows * lanes_of(A) + 255) / 256, LOSS_GROUPS); }
 // One workgroup, one launch: what the loss of a minibatch waits for is launches.
@@ -187,11 +211,11 @@ int64_t loss_workspace(int64_t rows, int A)
     return (int64_t)loss_groups(rows, A) * (LOSS_SUMS + A) * 8 + COUNT_GROUPS * 8;
 }
 
-template <typename TM, int AM, int GL, bool SHARED, bool PACKED> static int loss_go(LossDev p, hipStream_t st)
+template <typename TM, int AM, int GL, bool SHARED, bool LINEAR> static int loss_go(LossDev p, hipStream_t st)
 {
     if (loss_single(p.rows, p.A)) {
-        constexpr int BS = AM <= 2 ? 1024 : 512;                        // (the most threads that leave every value in a register)
-        hipLaunchKernelGGL((k_policy_loss<TM, AM, GL, SHARED, PACKED, BS>), dim3(1), dim3(BS), 0, st, p);
+        constexpr int BS = AM <= 2 && LINEAR ? 1024 : 512;              // (the most threads that leave every value in a register)
+        hipLaunchKernelGGL((k_policy_loss<TM, AM, GL, SHARED, LINEAR, BS>), dim3(1), dim3(BS), 0, st, p);
         LAUNCH_CHECK();
         return 0;
     }
@@ -201,7 +225,7 @@ template <typename TM, int AM, int GL, bool SHARED, bool PACKED> static int loss
         hipLaunchKernelGGL(k_mask_count, dim3(COUNT_GROUPS), dim3(256), 0, st, p.rows, p.n, p.mask, const_cast<int64_t *>(p.counts));
         LAUNCH_CHECK();
     }
-    hipLaunchKernelGGL((k_policy_loss<TM, AM, GL, SHARED, PACKED, 256>), dim3(groups), dim3(256), 0, st, p);
+    hipLaunchKernelGGL((k_policy_loss<TM, AM, GL, SHARED, LINEAR, 256>), dim3(groups), dim3(256), 0, st, p);
     LAUNCH_CHECK();
     hipLaunchKernelGGL((k_policy_loss_finish<TM, SHARED>), dim3(1), dim3(512), 0, st, p, groups);
     LAUNCH_CHECK();
@@ -210,11 +234,11 @@ template <typename TM, int AM, int GL, bool SHARED, bool PACKED> static int loss
 template <typename TM, int AM, int GL> static int loss_pick(const LossDev &p, bool shared, hipStream_t st)
 {
     const size_t row = sizeof(TM) * AM;
-    const auto packed_rows = [&](const Rows &t) { return AM == 1 || (t.sa == 1 && t.sb % AM == 0 && t.sn % AM == 0 && aligned(t.p, row)); };
-    const bool packed = p.A == AM * GL && packed_rows(p.mean) && (shared || packed_rows(p.log_std)) && aligned(p.dmean, row) && (shared || aligned(p.dstd, row));
-    if (packed) return shared ? loss_go<TM, AM, GL, true, true>(p, st) : loss_go<TM, AM, GL, false, true>(p, st);
-    if constexpr (AM > 1) return shared ? loss_go<TM, AM, GL, true, false>(p, st) : loss_go<TM, AM, GL, false, false>(p, st);
-    return -1;
+    const auto in_line = [&](const Rows &t, int A, size_t align) { return !t.p || ((A == 1 || t.sa == 1) && (t.sn == A || p.n == 1) && (t.sb == p.n * A || p.B == 1) && aligned(t.p, align)); };
+    const bool linear = p.A == AM * GL && in_line(p.mean, p.A, row) && (shared || in_line(p.log_std, p.A, row)) && in_line(p.old, 1, 4) && in_line(p.ref, 1, 4) &&
+                        in_line(p.adv, 1, 4) && in_line(p.mask, 1, 1) && aligned(p.dmean, row) && (shared || aligned(p.dstd, row));
+    if (linear) return shared ? loss_go<TM, AM, GL, true, true>(p, st) : loss_go<TM, AM, GL, false, true>(p, st);
+    return shared ? loss_go<TM, AM, GL, true, false>(p, st) : loss_go<TM, AM, GL, false, false>(p, st);
 }
 template <typename TM> static int loss_width(const LossDev &p, bool shared, hipStream_t st)
 {
@@ -233,6 +257,7 @@ int launch_policy_loss(const LossArgs &a, hipStream_t st)
     p.mean = a.mean; p.log_std = a.log_std; p.actions = a.actions; p.old = a.log_pi_old;
     p.ref = a.log_pi_ref.p ? a.log_pi_ref : a.log_pi_old;
     p.adv = a.adv; p.mask = a.mask; p.moments = a.adv_moments;
+    p.dlo = a.clip < 1.0 ? std::log1p(-a.clip) : -INFINITY; p.dhi = std::log1p(a.clip);       // (a ratio is never below 0)
     p.lo = 1.0 - a.clip; p.hi = 1.0 + a.clip; p.kl = a.kl_coef; p.ent = a.entropy_coef;
     p.loss = a.loss; p.stats = a.stats; p.dmean = a.dmean; p.dstd = a.dlog_std;
     if (!loss_single(p.rows, p.A)) {
@@ -246,7 +271,7 @@ int launch_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void 
 {
     const int64_t n = n_mean + n_std;
     if (n == 0) return 0;
-    const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 2048);
+    const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 1024);
     if (dtype == 0) hipLaunchKernelGGL(k_policy_loss_scale<float>, dim3(grid), dim3(256), 0, st, grad, n_mean, (float *)dmean, n_std, (float *)dlog_std);
     else hipLaunchKernelGGL(k_policy_loss_scale<bf16>, dim3(grid), dim3(256), 0, st, grad, n_mean, (bf16 *)dmean, n_std, (bf16 *)dlog_std);
     LAUNCH_CHECK();

@@ -8,64 +8,89 @@ mean and log_std are float32 or bfloat16, everything else float32.  No CPU fallb
 from __future__ import annotations
 
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from .recurrence import _DTYPES, _guard_leaves, _need, _on_device, _ptr, _workspace
+from .recurrence import _DTYPES, _FLAGS, _call, _guard_leaves, _need, _on_device, _ptr, _workspace
 
 STATS_FIELDS = ("gain", "kl", "entropy", "clipped", "ratio", "rows")
+_NO_ROWS = (0, 0, 0, 0)
+_pack_loss = struct.Struct("28q").pack                                  # struct asm_loss_rows
+_pack_act = struct.Struct("20q").pack                                   # struct asm_act_rows
 
 
-def _walk(t: torch.Tensor, lead: int) -> Optional[Tuple[int, int]]:
-    """Strides (sb, sn) that walk t's first `lead` axes as (all but the last, the last); None if there are none."""
-    shape, st = t.shape, t.stride()
-    sn = st[lead - 1] if lead else 0
+def _walk(shape, st, lead: int) -> Optional[Tuple[int, int]]:
+    """Strides (sb, sn) that walk a tensor's first `lead` axes as (all but the last, the last); None if there are none."""
+    if lead < 2:
+        return (0, st[0]) if lead else (0, 0)
+    if lead == 2:
+        return st[0], st[1]
     sb, span = 0, None
     for k in range(lead - 2, -1, -1):
         if shape[k] == 1:
             continue
         if span is None:
-            sb, span = st[k], st[k] * shape[k]
+            sb = st[k]
         elif st[k] != span:
             return None
-        else:
-            span = st[k] * shape[k]
-    return sb, sn
+        span = st[k] * shape[k]
+    return sb, st[lead - 1]
 
 
-def _rows(t: Optional[torch.Tensor], lead: int, axis: bool):
-    """(struct asm_rows, the tensor it points into) of an input."""
-    if t is None:
-        return _lib.AsmRows(None, 0, 0, 0), None
-    w = _walk(t, lead)
+def _rows(t: torch.Tensor, lead: int, axis: bool):
+    """One struct asm_rows (as four numbers) of an input, and the tensor it points into."""
+    st = t.stride()
+    w = _walk(t.shape, st, lead)
     if w is None:
         t = t.contiguous()
-        w = _walk(t, lead)
-    return _lib.AsmRows(t.data_ptr(), w[0], w[1], t.stride(-1) if axis else 0), t
+        st = t.stride()
+        w = _walk(t.shape, st, lead)
+    return (t.data_ptr(), w[0], w[1], st[-1] if axis else 0), t
+
+
+def _rows_std(t: torch.Tensor, lead: int, shared: bool):
+    return ((t.data_ptr(), 0, 0, t.stride(0)), t) if shared else _rows(t, lead, True)
 
 
 def _rows_out(t: torch.Tensor, lead: int, axis: bool, what: str):
-    w = _walk(t, lead)
-    _need(w is not None, f"{what} must be a tensor whose leading axes but the last can be walked with one stride")
-    _need(all(s != 0 for n, s in zip(t.shape, t.stride()) if n > 1), f"{what} must not be an expanded tensor")
-    return _lib.AsmRows(t.data_ptr(), w[0], w[1], t.stride(-1) if axis else 0)
+    shape, st = t.shape, t.stride()
+    w = _walk(shape, st, lead)
+    if w is None or 0 in st:
+        _need(w is not None, f"{what} must be a tensor whose leading axes but the last can be walked with one stride")
+        _need(all(s != 0 for n, s in zip(shape, st) if n > 1), f"{what} must not be an expanded tensor")
+    return t.data_ptr(), w[0], w[1], st[-1] if axis else 0
 
 
 def _dims(lead) -> Tuple[int, int]:
-    return (math.prod(lead[:-1]), lead[-1]) if lead else (1, 1)
+    return (lead[:-1].numel(), lead[-1]) if lead else (1, 1)
 
 
-def _check_policy(fn, mean, log_std, rows_of):
+def _policy_ok(mean, log_std, full, per_row) -> bool:
+    """Shapes, types and devices of a policy operator's tensors: full ones like mean, per_row ones without its last axis."""
+    shape, dt, dev = mean.shape, mean.dtype, mean.device
+    if not (shape and 1 <= shape[-1] <= 32 and dt in _DTYPES and log_std.dtype == dt and log_std.device == dev and dev.type == "cuda" and
+            (log_std.shape == shape[-1:] or log_std.shape == shape)):
+        return False
+    for t in full:
+        if t is not None and not (t.shape == shape and t.dtype == torch.float32 and t.device == dev):
+            return False
+    lead = shape[:-1]
+    for t in per_row:
+        if t is not None and not (t.shape == lead and t.dtype == torch.float32 and t.device == dev):
+            return False
+    return True
+
+
+def _explain_policy(fn, mean, log_std, full, per_row):
     _need(mean.dim() >= 1 and 1 <= mean.shape[-1] <= 32, f"{fn}: mean must be (..., A) with 1 to 32 action components, got {tuple(mean.shape)}")
     _need(mean.dtype in _DTYPES and log_std.dtype == mean.dtype, f"{fn}: mean and log_std must both be float32 or bfloat16, got {mean.dtype} and {log_std.dtype}")
-    shared = log_std.shape == mean.shape[-1:]
-    _need(shared or log_std.shape == mean.shape, f"{fn}: log_std must have the shape {tuple(mean.shape[-1:])} or {tuple(mean.shape)}")
-    for name, (t, axis) in rows_of.items():
-        want = mean.shape if axis else mean.shape[:-1]
-        _need(t is None or (t.shape == want and t.dtype == torch.float32), f"{fn}: {name} must be a float32 tensor of shape {tuple(want)}")
-    return shared
+    _need(log_std.shape == mean.shape[-1:] or log_std.shape == mean.shape, f"{fn}: log_std must have the shape {tuple(mean.shape[-1:])} or {tuple(mean.shape)}")
+    for names, want in ((full, mean.shape), (per_row, mean.shape[:-1])):
+        for name, t in names.items():
+            _need(t is None or (t.shape == want and t.dtype == torch.float32), f"{fn}: {name} must be a float32 tensor of shape {tuple(want)}")
 
 
 class _ClippedLoss(torch.autograd.Function):
@@ -88,32 +113,30 @@ class _ClippedLoss(torch.autograd.Function):
         tensors = ctx.saved_tensors                                     # (notices inputs overwritten since)
         grads, ctx.grads = ctx.grads, None
         dmean, dstd = grads if grads is not None else _loss(*tensors, *ctx.args)[2:]
-        with torch.cuda.device(dmean.device):
-            rc = _lib.load().asm_policy_loss_scale(_DTYPES[dmean.dtype], g.data_ptr(), dmean.numel(), dmean.data_ptr(), dstd.numel(), dstd.data_ptr(),
-                                                   torch.cuda.current_stream(dmean.device).cuda_stream)
-        _lib.check(rc, "asm_policy_loss_scale")
+        _call("asm_policy_loss_scale", dmean.device, _DTYPES[dmean.dtype], g.data_ptr(), dmean.numel(), dmean.data_ptr(), dstd.numel(), dstd.data_ptr())
         return (dmean, dstd) + none
 
 
 def _loss(mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl_coef, entropy_coef):
-    lib, dev = _lib.load(), mean.device
-    lead, A = mean.dim() - 1, mean.shape[-1]
-    B, n = _dims(mean.shape[:-1])
+    dev, shape, dt = mean.device, mean.shape, mean.dtype
+    lead, A = len(shape) - 1, shape[-1]
+    B, n = _dims(shape[:-1])
     out = torch.empty(7, dtype=torch.float32, device=dev)
-    loss, stats = out[0], out[1:]
-    dmean = torch.empty(mean.shape, dtype=mean.dtype, device=dev)
-    dstd = torch.empty(log_std.shape, dtype=mean.dtype, device=dev)
-    need = lib.asm_policy_loss_workspace(B * n, A)
+    dmean = torch.empty(shape, dtype=dt, device=dev)
+    dstd = torch.empty(log_std.shape, dtype=dt, device=dev)
+    need = _lib.load().asm_policy_loss_workspace(B * n, A)
     ws = _workspace(need, dev)
-    r_std = (_lib.AsmRows(log_std.data_ptr(), 0, 0, log_std.stride(0)), log_std) if shared else _rows(log_std, lead, True)
-    held = [_rows(mean, lead, True), r_std, _rows(actions, lead, True), _rows(old, lead, False), _rows(ref, lead, False),
-            _rows(adv, lead, False), _rows(mask, lead, False)]
-    with torch.cuda.device(dev):
-        rc = lib.asm_policy_loss(_DTYPES[mean.dtype], B, n, A, int(shared), *[h[0] for h in held], _ptr(moments), clip, kl_coef, entropy_coef,
-                                 loss.data_ptr(), stats.data_ptr(), dmean.data_ptr(), dstd.data_ptr(), _ptr(ws), max(need, 0),
-                                 torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "asm_policy_loss")
-    return loss, stats, dmean, dstd
+    r0, k0 = _rows(mean, lead, True)                                    # (k: the tensors a copy may have been made of)
+    r1, k1 = _rows_std(log_std, lead, shared)
+    r2, k2 = _rows(actions, lead, True)
+    r3, k3 = _rows(old, lead, False)
+    r4, k4 = _rows(ref, lead, False) if ref is not None else (_NO_ROWS, None)
+    r5, k5 = _rows(adv, lead, False)
+    r6, k6 = _rows(mask, lead, False) if mask is not None else (_NO_ROWS, None)
+    at = out.data_ptr()
+    _call("asm_policy_loss", dev, _DTYPES[dt], B, n, A, shared, _pack_loss(*r0, *r1, *r2, *r3, *r4, *r5, *r6), _ptr(moments), clip, kl_coef,
+          entropy_coef, at, at + 4, dmean.data_ptr(), dstd.data_ptr(), _ptr(ws), need)
+    return out[0], out[1:], dmean, dstd
 
 
 def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Tensor, log_pi_old: torch.Tensor, adv: torch.Tensor, *,
@@ -130,17 +153,31 @@ def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torc
     the same pass.  log_std: mean's shape, or (A,) for all rows.  adv_moments: the (mean, 1 / deviation) that
     advantages(..., moments=True) returns; A = (adv - mean) / deviation then, else A = adv.
     stats: 6 floats, STATS_FIELDS (means over the valid rows of min(..), e^D - 1 - D, H, rows cut off, q; the rows)."""
+    dev, lead = mean.device, mean.shape[:-1]
+    if not (_policy_ok(mean, log_std, (actions,), (log_pi_old, log_pi_ref, adv)) and
+            (mask is None or (mask.shape == lead and mask.dtype in _FLAGS and mask.device == dev)) and
+            (adv_moments is None or (adv_moments.shape == (2,) and adv_moments.dtype == torch.float32 and adv_moments.device == dev)) and
+            0.0 < clip < math.inf and math.isfinite(kl_coef) and math.isfinite(entropy_coef) and
+            not (torch.is_grad_enabled() and (actions.requires_grad or log_pi_old.requires_grad or adv.requires_grad or
+                                              (log_pi_ref is not None and log_pi_ref.requires_grad) or
+                                              (adv_moments is not None and adv_moments.requires_grad)))):
+        _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv_moments, clip, kl_coef, entropy_coef)
+    shared = int(log_std.shape == mean.shape[-1:])
+    adv_moments = None if adv_moments is None else adv_moments.contiguous()
+    loss, stats = _ClippedLoss.apply(mean, log_std, actions, log_pi_old, log_pi_ref, adv, mask, adv_moments, shared, float(clip), float(kl_coef), float(entropy_coef))
+    return (_guard_leaves(loss, mean.device) if loss.requires_grad else loss), stats
+
+
+def _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv_moments, clip, kl_coef, entropy_coef):
     fn = "clipped_policy_loss"
-    shared = _check_policy(fn, mean, log_std, dict(actions=(actions, True), log_pi_old=(log_pi_old, False), log_pi_ref=(log_pi_ref, False), adv=(adv, False)))
-    _need(mask is None or (mask.shape == mean.shape[:-1] and mask.dtype in (torch.bool, torch.uint8)), f"{fn}: mask must be a bool or uint8 tensor of shape {tuple(mean.shape[:-1])}")
+    _explain_policy(fn, mean, log_std, dict(actions=actions), dict(log_pi_old=log_pi_old, log_pi_ref=log_pi_ref, adv=adv))
+    _need(mask is None or (mask.shape == mean.shape[:-1] and mask.dtype in _FLAGS), f"{fn}: mask must be a bool or uint8 tensor of shape {tuple(mean.shape[:-1])}")
     _need(adv_moments is None or (adv_moments.shape == (2,) and adv_moments.dtype == torch.float32), f"{fn}: adv_moments must be two float32 numbers")
     _need(0.0 < clip < math.inf and math.isfinite(kl_coef) and math.isfinite(entropy_coef), f"{fn}: clip must be positive, the coefficients finite")
     for name, t in (("actions", actions), ("log_pi_old", log_pi_old), ("log_pi_ref", log_pi_ref), ("adv", adv), ("adv_moments", adv_moments)):
         _need(t is None or not (t.requires_grad and torch.is_grad_enabled()), f"{fn}: no gradient for {name}: pass it detached")
     _on_device(fn, mean.device, log_std, actions, log_pi_old, log_pi_ref, adv, mask, adv_moments)
-    adv_moments = None if adv_moments is None else adv_moments.contiguous()
-    loss, stats = _ClippedLoss.apply(mean, log_std, actions, log_pi_old, log_pi_ref, adv, mask, adv_moments, shared, float(clip), float(kl_coef), float(entropy_coef))
-    return (_guard_leaves(loss, mean.device) if loss.requires_grad else loss), stats
+    raise ValueError(f"{fn}: bad arguments")
 
 
 @torch.no_grad()
@@ -160,23 +197,25 @@ def gaussian_log_pi(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Te
 
 
 def _act(fn, mean, log_std, noise, actions, log_pi):
-    shared = _check_policy(fn, mean, log_std, dict(noise=(noise, True), actions=(actions, True), log_pi=(log_pi, False)))
-    dev, lead, A = mean.device, mean.dim() - 1, mean.shape[-1]
-    _on_device(fn, dev, log_std, noise, actions, log_pi)
-    B, n = _dims(mean.shape[:-1])
+    if not _policy_ok(mean, log_std, (noise, actions), (log_pi,)):
+        _explain_policy(fn, mean, log_std, dict(noise=noise, actions=actions), dict(log_pi=log_pi))
+        _on_device(fn, mean.device, log_std, noise, actions, log_pi)
+        raise ValueError(f"{fn}: bad arguments")
+    dev, shape, dt = mean.device, mean.shape, mean.dtype
+    lead, A = len(shape) - 1, shape[-1]
+    B, n = _dims(shape[:-1])
     if actions is None:
-        actions = torch.empty(mean.shape, dtype=torch.float32, device=dev)
+        actions = torch.empty(shape, dtype=torch.float32, device=dev)
     if log_pi is None:
-        log_pi = torch.empty(mean.shape[:-1], dtype=torch.float32, device=dev)
+        log_pi = torch.empty(shape[:-1], dtype=torch.float32, device=dev)
     if noise is not None:
-        r_act = _rows_out(actions, lead, True, f"{fn}: actions")
+        r_act, k_act = _rows_out(actions, lead, True, "actions"), None
+        r_noise, k_noise = _rows(noise, lead, True)
     else:
-        r_act, held_act = _rows(actions, lead, True)
-    r_lp = _rows_out(log_pi, lead, False, f"{fn}: log_pi")
-    r_std = (_lib.AsmRows(log_std.data_ptr(), 0, 0, log_std.stride(0)), log_std) if shared else _rows(log_std, lead, True)
-    r_mean, r_noise = _rows(mean, lead, True), _rows(noise, lead, True)
-    with torch.cuda.device(dev):
-        rc = _lib.load().asm_gaussian_act(_DTYPES[mean.dtype], B, n, A, r_mean[0], r_std[0], r_noise[0], r_act, r_lp, torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "asm_gaussian_act")
-    torch.autograd.graph.increment_version([log_pi] if noise is None else [actions, log_pi])
+        r_act, k_act = _rows(actions, lead, True)
+        r_noise, k_noise = _NO_ROWS, None
+    r_mean, k_mean = _rows(mean, lead, True)
+    r_std, k_std = _rows_std(log_std, lead, log_std.shape == shape[-1:])
+    _call("asm_gaussian_act", dev, _DTYPES[dt], B, n, A, _pack_act(*r_mean, *r_std, *r_noise, *r_act, *_rows_out(log_pi, lead, False, "log_pi")))
+    torch.autograd.graph.increment_version((log_pi,) if noise is None else (actions, log_pi))
     return actions, log_pi

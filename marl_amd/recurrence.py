@@ -16,6 +16,8 @@ import torch
 from . import _lib
 
 _DTYPES = {torch.float32: _lib.SEQ_F32, torch.bfloat16: _lib.SEQ_BF16}
+_FLAGS = (torch.bool, torch.uint8)
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _need(ok: bool, msg: str) -> None:
@@ -49,11 +51,25 @@ def _workspace(nbytes: int, device) -> Optional[torch.Tensor]:
     return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes > 0 else None
 
 
+def _call(name: str, dev: torch.device, *args) -> None:
+    """One entry point of the library on dev's current stream (its last argument).  A small call is bound by what Python does
+    around it: the device is only switched when it is not the current one, and the stream's handle is asked for
+    as a number (2.5 us less than through a torch.cuda.Stream object)."""
+    fn, index = getattr(_lib.load(), name), dev.index
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _lib.check(rc, name)
+
+
 def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
     """A leaf's accumulation node belongs to the stream it was first used on and lives as long as any graph that uses the
     leaf; a backward pass captured into a HIP graph would have to join that other stream, which ends the process.
     The node remembers its stream (in its own metadata, gone with the node), and such a capture is refused."""
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = _raw_stream(device.index)
     for node, _ in out.grad_fn.next_functions:
         if type(node).__name__ == "AccumulateGrad":
             first = node.metadata.setdefault("marl_amd_stream", stream)
@@ -63,31 +79,25 @@ def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
     return out
 
 
-def _check_scan(gate, x, h0, resets, lengths, batch_first):
+def _explain_scan(gate, x, h0, resets, lengths, B, D):
     fn = "gated_scan"
     _need(gate.dim() == 3 and gate.shape == x.shape, f"{fn}: gate and x must have one shape of three axes, got {tuple(gate.shape)} and {tuple(x.shape)}")
     _need(gate.dtype in _DTYPES and x.dtype == gate.dtype, f"{fn}: gate and x must both be float32 or bfloat16, got {gate.dtype} and {x.dtype}")
-    T, B, D = (gate.shape[1], gate.shape[0], gate.shape[2]) if batch_first else gate.shape
     _need(h0 is None or (h0.shape == (B, D) and h0.dtype == torch.float32), f"{fn}: h0 must be a float32 tensor of shape {(B, D)}")
-    _need(resets is None or (resets.shape == gate.shape[:2] and resets.dtype in (torch.bool, torch.uint8)),
+    _need(resets is None or (resets.shape == gate.shape[:2] and resets.dtype in _FLAGS),
           f"{fn}: resets must be a bool or uint8 tensor of shape {tuple(gate.shape[:2])}")
     _need(lengths is None or (lengths.shape == (B,) and lengths.dtype == torch.int32), f"{fn}: lengths must be an int32 tensor of shape {(B,)}")
     _on_device(fn, gate.device, x, h0, resets, lengths)
-    return T, B, D
 
 
 def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D):
-    lib = _lib.load()
-    h = torch.empty(gate.shape, dtype=gate.dtype, device=gate.device)
-    last = torch.empty(B, D, dtype=torch.float32, device=gate.device)
-    dt = _DTYPES[gate.dtype]
-    with torch.cuda.device(gate.device):
-        need = lib.asm_gated_scan_workspace(dt, T, B, D)
-        ws = _workspace(need, gate.device)
-        rc = lib.asm_gated_scan_forward(dt, T, B, D, *_tb(gate, batch_first), *_tb(x, batch_first), _ptr(h0), *_tb(resets, batch_first),
-                                        _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(ws), max(need, 0),
-                                        torch.cuda.current_stream(gate.device).cuda_stream)
-    _lib.check(rc, "asm_gated_scan_forward")
+    dev, dt = gate.device, _DTYPES[gate.dtype]
+    h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
+    last = torch.empty((B, D), dtype=torch.float32, device=dev)
+    need = _lib.load().asm_gated_scan_workspace(dt, T, B, D)
+    ws = _workspace(need, dev)
+    _call("asm_gated_scan_forward", dev, dt, T, B, D, *_tb(gate, batch_first), *_tb(x, batch_first), _ptr(h0), *_tb(resets, batch_first),
+          _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(ws), need)
     return h, last
 
 
@@ -105,21 +115,16 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         gate, x, h, h0, resets, lengths = ctx.saved_tensors
         T, B, D = ctx.dims
-        bf, dev = ctx.batch_first, gate.device
-        lib = _lib.load()
+        bf, dev, dt = ctx.batch_first, gate.device, _DTYPES[gate.dtype]
         dh = None if dh is None else _dense(dh)
         dlast = None if dlast is None else dlast.contiguous()
         dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         dx = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
-        dh0 = torch.empty(B, D, dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
-        dt = _DTYPES[gate.dtype]
-        with torch.cuda.device(dev):
-            need = lib.asm_gated_scan_workspace(dt, T, B, D)
-            ws = _workspace(need, dev)
-            rc = lib.asm_gated_scan_backward(dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf),
-                                             _ptr(lengths), *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0),
-                                             _ptr(ws), max(need, 0), torch.cuda.current_stream(dev).cuda_stream)
-        _lib.check(rc, "asm_gated_scan_backward")
+        dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
+        need = _lib.load().asm_gated_scan_workspace(dt, T, B, D)
+        ws = _workspace(need, dev)
+        _call("asm_gated_scan_backward", dev, dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf), _ptr(lengths),
+              *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0), _ptr(ws), need)
         return dgate, dx, dh0, None, None, None, None
 
 
@@ -133,7 +138,13 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     zero in front of that step, whatever it holds, and no gradient passes.  lengths: (B,) int32, clamped to 0..T: steps from
     there on are no part of the sequence; h and the gradients are zero there, and what gate and x hold does not matter.
     Sequences may be of length 0."""
-    T, B, D = _check_scan(gate, x, h0, resets, lengths, batch_first)
+    shape, dev = gate.shape, gate.device
+    T, B, D = shape if len(shape) == 3 and not batch_first else (shape[1], shape[0], shape[2]) if len(shape) == 3 else (0, 0, 0)
+    if not (len(shape) == 3 and x.shape == shape and gate.dtype in _DTYPES and x.dtype == gate.dtype and dev.type == "cuda" and x.device == dev and
+            (h0 is None or (h0.shape == (B, D) and h0.dtype == torch.float32 and h0.device == dev)) and
+            (resets is None or (resets.shape == shape[:2] and resets.dtype in _FLAGS and resets.device == dev)) and
+            (lengths is None or (lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.device == dev))):
+        _explain_scan(gate, x, h0, resets, lengths, B, D)
     gate, x = _dense(gate), _dense(x)
     h0 = None if h0 is None else h0.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
@@ -148,34 +159,41 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
     """One step of the memory in a rollout, without gradients: state (B, D) float32, contiguous, is updated in place, the
     new state is returned in gate's type (in `out` if given; it may be gate or x itself, not the state).  reset: (B,) bool or uint8; where
     set, the state counts as zero first."""
+    shape, dt, dev = gate.shape, gate.dtype, gate.device
+    D = shape[-1] if shape else 0
+    if out is None and dev.type == "cuda":
+        out = torch.empty(shape, dtype=dt, device=dev)
+    if not (len(shape) == 2 and x.shape == shape and state.shape == shape and dt in _DTYPES and x.dtype == dt and state.dtype == torch.float32 and
+            state.is_contiguous() and not ((state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled()) and
+            (reset is None or (reset.shape == shape[:1] and reset.dtype in _FLAGS and reset.device == dev)) and dev.type == "cuda" and
+            x.device == dev and state.device == dev and out.device == dev and out.shape == shape and out.dtype == dt and
+            (D <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= D) and (out.data_ptr() != state.data_ptr() or shape.numel() == 0)):
+        _explain_step(gate, x, state, reset, out)
+    gate, x = _dense(gate), _dense(x)
+    _call("asm_gated_scan_step", dev, _DTYPES[dt], shape[0], D, gate.data_ptr(), gate.stride(0), x.data_ptr(), x.stride(0), state.data_ptr(),
+          _ptr(reset), 0 if reset is None else reset.stride(0), out.data_ptr(), out.stride(0))
+    torch.autograd.graph.increment_version((state, out))                # (written behind autograd's back)
+    return out
+
+
+def _explain_step(gate, x, state, reset, out):
     fn = "gated_scan_step"
     _need(gate.dim() == 2 and gate.shape == x.shape == state.shape, f"{fn}: gate, x and state must have one shape of two axes")
     _need(gate.dtype in _DTYPES and x.dtype == gate.dtype, f"{fn}: gate and x must both be float32 or bfloat16, got {gate.dtype} and {x.dtype}")
     _need(state.dtype == torch.float32 and state.is_contiguous(), f"{fn}: state must be a contiguous float32 tensor")
     _need(not (state.requires_grad and torch.is_grad_enabled()), f"{fn}: the state is updated in place and cannot require a gradient")
     B, D = gate.shape
-    _need(reset is None or (reset.shape == (B,) and reset.dtype in (torch.bool, torch.uint8)), f"{fn}: reset must be a bool or uint8 tensor of shape {(B,)}")
+    _need(reset is None or (reset.shape == (B,) and reset.dtype in _FLAGS), f"{fn}: reset must be a bool or uint8 tensor of shape {(B,)}")
     _need(out is None or (out.shape == gate.shape and out.dtype == gate.dtype and (D <= 1 or out.stride(1) == 1) and (B <= 1 or out.stride(0) >= D)
                           and not (out.requires_grad and torch.is_grad_enabled())),
           f"{fn}: out must be a tensor of gate's shape and type with contiguous rows that do not overlap")
-    dev = gate.device
-    _on_device(fn, dev, x, state, reset, out)
-    gate, x = _dense(gate), _dense(x)
-    if out is None:
-        out = torch.empty(B, D, dtype=gate.dtype, device=dev)
-    _need(B * D == 0 or out.data_ptr() != state.data_ptr(), f"{fn}: out and state must be two tensors")
-    with torch.cuda.device(dev):
-        rc = _lib.load().asm_gated_scan_step(_DTYPES[gate.dtype], B, D, gate.data_ptr(), gate.stride(0), x.data_ptr(), x.stride(0), state.data_ptr(),
-                                             _ptr(reset), 0 if reset is None else reset.stride(0), out.data_ptr(), out.stride(0),
-                                             torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "asm_gated_scan_step")
-    torch.autograd.graph.increment_version([state, out])                # (written behind autograd's back)
-    return out
+    _on_device(fn, gate.device, x, state, reset, out)
+    raise ValueError(f"{fn}: out and state must be two tensors")
 
 
 def _time_rows(t: torch.Tensor) -> torch.Tensor:
     """t with every time step contiguous (steps may lie any distance apart)."""
-    return t if t.shape[0] == 0 or t[0].is_contiguous() else t.contiguous()
+    return t if t.is_contiguous() or t[0].is_contiguous() else t.contiguous()
 
 
 @torch.no_grad()
@@ -190,29 +208,34 @@ def advantages(rewards: torch.Tensor, values: torch.Tensor, *, dones: Optional[t
     lengths: (E,) int32, clamped to 0..T: environment e ends after lengths[e] steps, values[lengths[e]] behind its last one;
     beyond it both results are zero.  moments=True also returns the two numbers clipped_policy_loss normalises with:
     mean and 1 / (standard deviation + 1e-8) of the advantages of all steps (population deviation), as a float32 tensor."""
-    fn = "advantages"
-    _need(rewards.dim() >= 2 and rewards.shape[0] >= 1 and rewards.numel() > 0, f"{fn}: rewards must be a non-empty (T, E, ...) tensor")
-    T, E = rewards.shape[0], rewards.shape[1]
-    _need(tuple(values.shape) == (T + 1,) + tuple(rewards.shape[1:]), f"{fn}: values must have the shape {(T + 1,) + tuple(rewards.shape[1:])}")
-    _need(rewards.dtype == torch.float32 and values.dtype == torch.float32, f"{fn}: rewards and values must be float32")
-    _need(dones is None or (dones.shape == rewards.shape and dones.dtype in (torch.bool, torch.uint8)), f"{fn}: dones must be a bool or uint8 tensor of rewards' shape")
-    _need(lengths is None or (lengths.shape == (E,) and lengths.dtype == torch.int32), f"{fn}: lengths must be an int32 tensor of shape {(E,)}")
-    _need(0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0, f"{fn}: gamma and lam must lie in [0, 1]")
-    dev = rewards.device
-    _on_device(fn, dev, values, dones, lengths)
+    shape, dev = rewards.shape, rewards.device
+    if not (len(shape) >= 2 and shape.numel() > 0 and values.shape == (shape[0] + 1,) + shape[1:] and rewards.dtype == torch.float32 and
+            values.dtype == torch.float32 and (dones is None or (dones.shape == shape and dones.dtype in _FLAGS and dones.device == dev)) and
+            (lengths is None or (lengths.shape == shape[1:2] and lengths.dtype == torch.int32 and lengths.device == dev)) and
+            0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0 and dev.type == "cuda" and values.device == dev):
+        _explain_advantages(rewards, values, dones, lengths, gamma, lam)
+    T, E = shape[0], shape[1]
+    D = shape.numel() // (T * E)
     rewards, values = _time_rows(rewards), _time_rows(values)
     dones = None if dones is None else _time_rows(dones)
     lengths = None if lengths is None else lengths.contiguous()
-    adv = torch.empty(rewards.shape, dtype=torch.float32, device=dev)
-    ret = torch.empty(rewards.shape, dtype=torch.float32, device=dev)
+    adv = torch.empty(shape, dtype=torch.float32, device=dev)
+    ret = torch.empty(shape, dtype=torch.float32, device=dev)
     mom = torch.empty(2, dtype=torch.float32, device=dev) if moments else None
-    D = rewards[0].numel() // E
-    lib = _lib.load()
-    with torch.cuda.device(dev):
-        need = lib.asm_advantages_workspace(T, E, D)
-        ws = _workspace(need, dev)
-        rc = lib.asm_advantages_f32(T, E, D, rewards.data_ptr(), rewards.stride(0), values.data_ptr(), values.stride(0), _ptr(dones),
-                                    0 if dones is None else dones.stride(0), _ptr(lengths), float(gamma), float(lam), adv.data_ptr(),
-                                    ret.data_ptr(), _ptr(mom), _ptr(ws), max(need, 0), torch.cuda.current_stream(dev).cuda_stream)
-    _lib.check(rc, "asm_advantages_f32")
+    need = _lib.load().asm_advantages_workspace(T, E, D)
+    ws = _workspace(need, dev)
+    _call("asm_advantages_f32", dev, T, E, D, rewards.data_ptr(), rewards.stride(0), values.data_ptr(), values.stride(0), _ptr(dones),
+          0 if dones is None else dones.stride(0), _ptr(lengths), gamma, lam, adv.data_ptr(), ret.data_ptr(), _ptr(mom), _ptr(ws), need)
     return (adv, ret, mom) if moments else (adv, ret)
+
+
+def _explain_advantages(rewards, values, dones, lengths, gamma, lam):
+    fn = "advantages"
+    _need(rewards.dim() >= 2 and rewards.numel() > 0, f"{fn}: rewards must be a non-empty (T, E, ...) tensor")
+    T, E = rewards.shape[0], rewards.shape[1]
+    _need(tuple(values.shape) == (T + 1,) + tuple(rewards.shape[1:]), f"{fn}: values must have the shape {(T + 1,) + tuple(rewards.shape[1:])}")
+    _need(rewards.dtype == torch.float32 and values.dtype == torch.float32, f"{fn}: rewards and values must be float32")
+    _need(dones is None or (dones.shape == rewards.shape and dones.dtype in _FLAGS), f"{fn}: dones must be a bool or uint8 tensor of rewards' shape")
+    _need(lengths is None or (lengths.shape == (E,) and lengths.dtype == torch.int32), f"{fn}: lengths must be an int32 tensor of shape {(E,)}")
+    _need(0.0 <= gamma <= 1.0 and 0.0 <= lam <= 1.0, f"{fn}: gamma and lam must lie in [0, 1]")
+    _on_device(fn, rewards.device, values, dones, lengths)

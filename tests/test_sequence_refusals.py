@@ -1,6 +1,6 @@
 """What the sequence operators refuse, at the Python entry points (before any device is asked for) and at the C ABI
 (before anything is launched).  Runs on the CPU."""
-import ctypes as C
+import struct
 
 import pytest
 import torch
@@ -132,12 +132,14 @@ def test_c_abi_refuses_before_it_launches():
     adv = lambda T=T, g=0.9, r=p, ws=None, n=0: lib.asm_advantages_f32(T, B, D, r, 0, p, 0, None, 0, None, g, 0.9, p, p, None, ws, n, None)  # noqa: E731
     for kw, msg in ((dict(T=0), "no steps"), (dict(g=1.5), "gamma"), (dict(g=float("nan")), "gamma"), (dict(r=None), "NULL"), (dict(T=100000), "workspace")):
         assert adv(ws=None, **kw) != 0 and msg in _msg(lib), (kw, _msg(lib))
-    R = lambda ptr=p: C.byref(_lib.AsmRows(ptr, 0, 0, 0))  # noqa: E731
+    R = lambda *ptrs: struct.pack(f"{4 * len(ptrs)}q", *(v for q in ptrs for v in (q, 0, 0, 0)))  # noqa: E731
     loss = lambda B=1, n=5, A=2, mean=p, std=p, clip=0.2, dm=p, nb=0: lib.asm_policy_loss(  # noqa: E731
-        0, B, n, A, 1, R(mean), R(std), R(), R(), R(None), R(), R(None), None, clip, 0.0, 0.0, p, p, dm, p, None, nb, None)
-    for kw, msg in ((dict(A=0), "A = 0"), (dict(A=33), "A = 33"), (dict(mean=None), "NULL"), (dict(std=None), "NULL"), (dict(dm=None), "NULL"),
+        0, B, n, A, 1, R(mean, std, p, p, 0, p, 0), None, clip, 0.0, 0.0, p, p, dm, p, None, nb, None)
+    for kw, msg in ((dict(A=0), "A = 0"), (dict(A=33), "A = 33"), (dict(mean=0), "NULL"), (dict(std=0), "NULL"), (dict(dm=None), "NULL"),
                     (dict(clip=-1.0), "clip"), (dict(clip=float("nan")), "clip"), (dict(n=1 << 20), "workspace"), (dict(B=1 << 20, n=1 << 20), "too large")):
         assert loss(**kw) != 0 and msg in _msg(lib), (kw, _msg(lib))
     assert lib.asm_policy_loss_scale(0, None, 4, p, 0, None, None) != 0
-    assert lib.asm_gaussian_act(0, 1, 5, 2, R(), R(), R(), R(None), R(), None) != 0 and "NULL" in _msg(lib)
-    assert lib.asm_gaussian_act(3, 1, 5, 2, R(), R(), R(), R(), R(), None) != 0 and "dtype" in _msg(lib)
+    assert lib.asm_policy_loss(0, 1, 5, 2, 1, None, None, 0.2, 0.0, 0.0, p, p, p, p, None, 0, None) != 0 and "NULL" in _msg(lib)
+    assert lib.asm_gaussian_act(0, 1, 5, 2, R(p, p, p, 0, p), None) != 0 and "NULL" in _msg(lib)
+    assert lib.asm_gaussian_act(0, 1, 5, 2, None, None) != 0 and "NULL" in _msg(lib)
+    assert lib.asm_gaussian_act(3, 1, 5, 2, R(p, p, p, p, p), None) != 0 and "dtype" in _msg(lib)
