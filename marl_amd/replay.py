@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from . import _lib
+from .recurrence import advantages
 
 
 class ReplayBufferAgent:
@@ -123,7 +124,7 @@ class DeviceReplay:
     episodes) is left out until its last step.
     """
 
-    def __init__(self, env, episode_length: int, slots: int, seed: int = 0):
+    def __init__(self, env, episode_length: int, slots: int, seed: int = 0, log_pi: bool = False):
         self.env = env
         self.lib = _lib.load()
         self.T, self.S = int(episode_length), int(slots)
@@ -133,6 +134,8 @@ class DeviceReplay:
         self.act_ring = torch.zeros(self.S, self.T, E, 2, n, **f32)
         self.prior_ring = torch.zeros(self.S, self.T, E, 2, n, **f32) if env.training_method == "llm_rl" else None
         self.rew_ring = torch.zeros(self.S, self.T, E, 1, n, **f32)
+        # log_pi=True: the log-probabilities of the actions (the log_pi column of buffer_agent.py:54-60), for on-policy training
+        self.log_pi_ring = torch.zeros(self.S, self.T, E, n, **f32) if log_pi else None
         self.slot, self.t = -1, 0
         self.complete = [False] * self.S                            # per slot: holds one whole episode
         self.seed, self.draws = int(seed), 0
@@ -155,6 +158,21 @@ class DeviceReplay:
         """Where this step's actions are stored; pass it to env.step() after filling it."""
         self._point_outputs()
         return self.act_ring[self.slot, self.t]
+
+    def log_pi_slot(self) -> torch.Tensor:
+        """Where the log-probabilities of this step's actions are stored: (E, n_a)."""
+        if self.log_pi_ring is None:
+            raise RuntimeError("constructed without log_pi=True")
+        return self.log_pi_ring[self.slot, self.t]
+
+    def advantages(self, values: torch.Tensor, slot: Optional[int] = None, gamma: float = 0.95, lam: float = 0.95):
+        """Advantages and returns of a complete episode slot (the last one written by default) from the critic's values (T + 1, E,
+        n_a): (adv, ret, moments), the first two (T, E, n_a).  Episodes of this environment are never done early
+        (assembly.py:475-477)."""
+        slot = self.slot if slot is None else int(slot)
+        if not 0 <= slot < self.S or not self.complete[slot]:
+            raise RuntimeError(f"slot {slot} holds no complete episode")
+        return advantages(self.rew_ring[slot].squeeze(2), values, gamma=gamma, lam=lam, moments=True)
 
     def _point_outputs(self) -> None:
         e = self.env

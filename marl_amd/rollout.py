@@ -1,7 +1,8 @@
 """The rollout / update loop of train_assembly.py:89-161 on the device: policy forward for all
 E x n_a agents in one matmul chain, BatchedAssemblyEnv.step, DeviceReplay as the push, and a DDPG
 update that follows maddpg.py:99-199.  PyTorch provides the networks and optimisers; the environment
-and the replay gather are the HIP library.
+and the replay gather are the HIP library.  ClippedPolicyLearner and train_on_policy() train a policy with a memory on whole episodes
+instead, through the library's sequence operators (recurrence.py, policy_loss.py).
 """
 from __future__ import annotations
 
@@ -14,6 +15,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .batched import BatchedAssemblyEnv
+from .policy_loss import clipped_policy_loss, gaussian_act
+from .recurrence import gated_scan, gated_scan_step
 from .replay import DeviceReplay
 from .sharding import all_reduce_sum, reduce_episode_stats
 
@@ -37,6 +40,36 @@ class MLPNetwork(nn.Module):
         return torch.tanh(out) if self.constrain_out else out
 
 
+class MemoryPolicy(nn.Module):
+    """The policy network of networks.py:6-44 with a memory in the place of its middle layer (an agent sees its neighbourhood
+    only, and what it saw before is gone otherwise): linear, leaky_relu, linear to (gate, x), gated memory, linear, tanh;
+    and the logarithm of the actions' standard deviation, one for each component."""
+
+    def __init__(self, input_dim: int, out_dim: int, hidden_dim: int = 64, init_std: float = 0.5):
+        super().__init__()
+        self.fc1 = nn.Linear(input_dim, hidden_dim)
+        self.fc2 = nn.Linear(hidden_dim, 2 * hidden_dim)
+        self.fc4 = nn.Linear(hidden_dim, out_dim)
+        self.log_std = nn.Parameter(torch.full((out_dim,), math.log(init_std)))
+        self.hidden_dim = hidden_dim
+        with torch.no_grad():
+            self.fc2.bias[:hidden_dim] += 2.0                              # gates start at a memory of about eight steps
+
+    def _inputs(self, rows):
+        return self.fc2(F.leaky_relu(self.fc1(rows))).chunk(2, dim=-1)
+
+    def forward(self, rows, h0=None, resets=None):
+        """rows (T, B, obs_dim) -> (mean of the actions (T, B, out_dim), state behind the last step (B, hidden_dim))."""
+        gate, x = self._inputs(rows)
+        h, last = gated_scan(gate, x, h0, resets=resets)
+        return torch.tanh(self.fc4(h)), last
+
+    def step(self, rows, state, reset=None):
+        """One rollout step: rows (B, obs_dim) -> mean of the actions (B, out_dim); state (B, hidden_dim) is updated in place."""
+        gate, x = self._inputs(rows)
+        return torch.tanh(self.fc4(gated_scan_step(gate, x, state, reset=reset)))
+
+
 class _FlatGrads:
     """All gradients of a module as views into one contiguous buffer, so that a data-parallel step is ONE
     all-reduce per optimiser step (the reference's helper, misc.py:33-38, issues one per parameter tensor)."""
@@ -55,6 +88,15 @@ class _FlatGrads:
     def average(self, group=None) -> None:
         all_reduce_sum(self.flat, group)
         self.flat.div_(dist.get_world_size(group))
+
+
+def _obs_rows(obs: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """(E, obs_dim, n_a) float32 frames on the device -> rows (E * n_a, obs_dim), one per agent (asm_obs_rows_f32)."""
+    from . import _lib
+    E, d, n = obs.shape
+    _lib.check(_lib.load().asm_obs_rows_f32(E, n, d, obs.data_ptr(), rows.data_ptr(),
+                                            torch.cuda.current_stream(obs.device).cuda_stream), "asm_obs_rows_f32")
+    return rows
 
 
 class DDPGLearner:
@@ -148,14 +190,12 @@ class DDPGLearner:
         E, d, n = obs.shape
         if not (obs.is_cuda and obs.is_contiguous() and obs.dtype is torch.float32):
             return obs.transpose(1, 2).reshape(E * n, d)
-        from . import _lib
-        key = (E, d, n, obs.device)
+        # (a buffer for each stream as well: shards of one size act on streams of their own, at the same time)
+        key = (E, d, n, obs.device, torch.cuda.current_stream(obs.device).cuda_stream)
         buf = self._row_bufs.get(key)
         if buf is None:
             buf = self._row_bufs[key] = torch.empty(E * n, d, dtype=torch.float32, device=obs.device)
-        _lib.check(_lib.load().asm_obs_rows_f32(E, n, d, obs.data_ptr(), buf.data_ptr(),
-                                                torch.cuda.current_stream(obs.device).cuda_stream), "asm_obs_rows_f32")
-        return buf
+        return _obs_rows(obs, buf)
 
     def policy_changed(self) -> None:
         """Tell the learner that the policy's weights were changed by something Python did not see run (a replayed HIP
@@ -238,18 +278,120 @@ class DDPGLearner:
         self.niter += 1
 
 
+class ClippedPolicyLearner:
+    """On-policy counterpart of DDPGLearner for the same environments, replay and loops: a Gaussian policy with a memory, trained
+    on whole episodes with the clipped policy loss, and a critic of the state alone whose values give the advantages.
+
+    run_episode() with a DeviceReplay(..., log_pi=True) records an episode under it, train_on_policy() updates it from that
+    episode.  Memories are kept for each group of environments (by its first global id) and cleared by begin_episode()."""
+
+    def __init__(self, obs_dim: int, act_dim: int = 2, hidden_dim: int = 256, lr_actor: float = 3e-4, lr_critic: float = 1e-3,
+                 gamma: float = 0.95, lam: float = 0.95, clip: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
+                 init_std: float = 0.5, device="cuda"):
+        self.policy = MemoryPolicy(obs_dim, act_dim, hidden_dim, init_std).to(device)
+        self.critic = MLPNetwork(obs_dim, 1, hidden_dim).to(device)
+        self.policy_optimizer = torch.optim.Adam(self.policy.parameters(), lr_actor)
+        self.critic_optimizer = torch.optim.Adam(self.critic.parameters(), lr_critic)
+        self.gamma, self.lam, self.clip, self.kl_coef, self.entropy_coef = gamma, lam, clip, kl_coef, entropy_coef
+        self.fused_policy, self._explore_step = None, 0                    # (read by the loops written for DDPGLearner)
+        self._row_bufs = {}
+        self._states = {}
+
+    _agent_rows = DDPGLearner._agent_rows
+
+    def begin_episode(self) -> None:
+        """All memories empty: call before an episode's first act()."""
+        self._states.clear()
+
+    @torch.no_grad()
+    def act(self, obs: torch.Tensor, out: torch.Tensor, noise_scale: float = 0.0, epsilon: float = 0.0,
+            generator: Optional[torch.Generator] = None, env0: int = 0, explore_step: Optional[int] = None,
+            log_pi: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """obs (E, obs_dim, n_a) -> out (E, act_dim, n_a), the memories of environments env0 .. env0 + E - 1 one step further.
+        noise_scale > 0: actions drawn from the policy (with its own deviation; epsilon belongs to the other learner), their
+        log-probabilities written to log_pi (E, n_a); 0: the policy's mean."""
+        E, _, n = obs.shape
+        state = self._states.get(env0)
+        if state is None:
+            state = self._states[env0] = torch.zeros(E * n, self.policy.hidden_dim, dtype=torch.float32, device=obs.device)
+        mean = self.policy.step(self._agent_rows(obs), state).view(E, n, -1)
+        if noise_scale > 0.0:
+            noise = torch.randn(mean.shape, device=mean.device, generator=generator)
+            gaussian_act(mean, self.policy.log_std, noise, actions=out.transpose(1, 2), log_pi=log_pi)
+        else:
+            out.copy_(mean.transpose(1, 2))
+        return out
+
+    def _rows(self, frames: torch.Tensor) -> torch.Tensor:
+        """(T, E, obs_dim, n_a) frames -> (T, E * n_a, obs_dim)"""
+        T, E, d, n = frames.shape
+        if frames.is_contiguous() and frames.is_cuda:                      # (rows of their own: a backward pass reads them later)
+            return _obs_rows(frames.view(T * E, d, n), torch.empty(T * E * n, d, dtype=torch.float32, device=frames.device)).view(T, E * n, d)
+        return frames.transpose(2, 3).reshape(T, E * n, d)
+
+    def update(self, frames, actions, log_pi, adv, ret, moments):
+        """One step of both optimisers on an episode of some environments: frames (T, E, obs_dim, n_a), actions (T, E, act_dim, n_a),
+        log_pi, adv and ret (T, E, n_a).  Returns (policy loss, critic loss, stats) as tensors (policy_loss.STATS_FIELDS)."""
+        T, E, _, n = frames.shape
+        rows = self._rows(frames)
+        mean, _ = self.policy(rows)
+        loss, stats = clipped_policy_loss(mean.view(T, E, n, -1), self.policy.log_std, actions.transpose(2, 3), log_pi, adv, adv_moments=moments,
+                                          clip=self.clip, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
+        self.policy_optimizer.zero_grad()
+        loss.backward()
+        self.policy_optimizer.step()
+        vf_loss = F.mse_loss(self.critic(rows).view(T, E, n), ret)
+        self.critic_optimizer.zero_grad()
+        vf_loss.backward()
+        self.critic_optimizer.step()
+        return loss.detach(), vf_loss.detach(), stats
+
+
+def train_on_policy(env: BatchedAssemblyEnv, learner: ClippedPolicyLearner, replay: DeviceReplay, epochs: int = 4, envs_per_batch: int = 64):
+    """The on-policy counterpart of train_phase(): `epochs` passes over the episode run_episode() left in the replay's current
+    slot, envs_per_batch environments at a time, in order.  Returns a (updates, 8) tensor: policy loss, critic loss and
+    policy_loss.STATS_FIELDS of each update; nothing is read back in between."""
+    k = replay.slot
+    if k < 0 or not replay.complete[k] or replay.log_pi_ring is None:
+        raise RuntimeError("train_on_policy needs a complete episode recorded with DeviceReplay(..., log_pi=True)")
+    T, E = replay.T, env.E
+    frames, acts, log_pi = replay.obs_ring[k], replay.act_ring[k], replay.log_pi_ring[k]
+    groups = [slice(e, min(e + envs_per_batch, E)) for e in range(0, E, envs_per_batch)]
+    values = torch.empty(T + 1, E, env.n_a, dtype=torch.float32, device=env.device)
+    with torch.no_grad():
+        for g in groups:
+            values[:, g] = learner.critic(learner._rows(frames[:, g])).view(T + 1, -1, env.n_a)
+    adv, ret, moments = replay.advantages(values, gamma=learner.gamma, lam=learner.lam)
+    out = []
+    for _ in range(epochs):
+        for g in groups:
+            loss, vf, stats = learner.update(frames[:T, g], acts[:, g], log_pi[:, g], adv[:, g], ret[:, g], moments)
+            out.append(torch.cat((loss.view(1), vf.view(1), stats)))
+    return torch.stack(out)
+
+
+def _log_pi_of(learner, replay):
+    """What act() of an on-policy learner also takes: where the step's log-probabilities go (nothing for the others)."""
+    return {"log_pi": replay.log_pi_slot()} if isinstance(learner, ClippedPolicyLearner) else {}
+
+
 def run_episode(env: BatchedAssemblyEnv, learner: DDPGLearner, replay: DeviceReplay, episode_length: int,
                 noise_scale: float = 0.9, epsilon: float = 0.1, generator: Optional[torch.Generator] = None):
     """train_assembly.py:99-135 for E environments: reset, episode_length steps of act -> step, the
     environment writing straight into the replay slot.  Returns the episode statistics
-    (mean reward, coverage, uniformity, contacts, distance to target — summarize() of the 8-vector)."""
+    (mean reward, coverage, uniformity, contacts, distance to target — summarize() of the 8-vector).
+    learner: a DDPGLearner, or a ClippedPolicyLearner with a DeviceReplay(..., log_pi=True)."""
+    if isinstance(learner, ClippedPolicyLearner):
+        if noise_scale <= 0.0:
+            raise ValueError("an on-policy episode is drawn from the policy: noise_scale must be positive")
+        learner.begin_episode()
     if hasattr(env, "envs"):
         return _run_episode_shards(env, learner, replay, episode_length, noise_scale, epsilon, generator)
     replay.begin_episode()
     obs = env.reset()
     for _ in range(episode_length):
         a = replay.action_slot()
-        learner.act(obs, a, noise_scale, epsilon, generator, env0=env.env_id_offset)
+        learner.act(obs, a, noise_scale, epsilon, generator, env0=env.env_id_offset, **_log_pi_of(learner, replay))
         obs = env.step(a)[0]
         replay.advance()
     return reduce_episode_stats(env.episode_stats())
@@ -271,10 +413,12 @@ def _run_episode_shards(shards, learner: DDPGLearner, replay: DeviceReplay, epis
     for _ in range(episode_length):
         a = replay.action_slot()
         learner._explore_step += 1
+        more = _log_pi_of(learner, replay)
         for k, (env, (first, count)) in enumerate(zip(shards.envs, shards.ranges)):
             ak = a[first:first + count]
+            mk = {name: t[first:first + count] for name, t in more.items()}
             with torch.cuda.stream(shards.streams[k]):
-                learner.act(obs[k], ak, noise_scale, epsilon, generator, env0=env.env_id_offset, explore_step=learner._explore_step)
+                learner.act(obs[k], ak, noise_scale, epsilon, generator, env0=env.env_id_offset, explore_step=learner._explore_step, **mk)
             obs[k] = env.step(ak, shards._stream_ptrs[k])[0]
         replay.advance()
     return reduce_episode_stats(shards.episode_stats())                # (the current stream waits for the shards here)
@@ -288,6 +432,8 @@ def eval_episode(env: BatchedAssemblyEnv, learner: DDPGLearner, episode_length: 
     process_shape), and the formation metrics of the current state are recorded (:155-170).
     Returns (metrics (episode_length, E, 5) float64 on the device, columns BatchedAssemblyEnv.METRIC_FIELDS,
     total reward per environment (E,))."""
+    if isinstance(learner, ClippedPolicyLearner):
+        learner.begin_episode()
     obs = env.reset()
     metrics = torch.empty(episode_length, env.E, 5, dtype=torch.float64, device=env.device)
     total = torch.zeros(env.E, dtype=torch.float64, device=env.device)
