@@ -3,6 +3,7 @@
 Bounds: seq_oracle.policy_loss's for the float32 arithmetic of a row, and the rounding of each result: half a step of its type,
 2^-24 for float32; a bfloat16 gradient is rounded from float32, 2^-8.  An upstream gradient other than 1 multiplies the
 stored one: once more the same."""
+import gc
 import math
 
 import pytest
@@ -10,6 +11,17 @@ import pytest
 import seq_oracle as so
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def no_garbage():
+    """A HIP graph that the garbage collector frees while another one is captured ends the process (its destructor may not
+    run then): none is left from tests before, and none to tests after."""
+    gc.collect()
+    yield
+    gc.collect()
+
+
 U = so.U
 
 
@@ -183,7 +195,7 @@ def test_actions_and_their_log_pi(torch_cuda, E, n, A, shared, dtype):
     assert torch.equal(plain, act) and torch.equal(lp2, got)
 
 
-def test_captured_graphs(torch_cuda):
+def test_captured_graphs(torch_cuda, no_garbage):
     torch = torch_cuda
     from marl_amd.policy_loss import clipped_policy_loss, gaussian_act
     c = _make(torch, (50, 200), 2, "float32", True, 8, True, 0.5)       # (several workgroups, a mask: a workspace is in use)

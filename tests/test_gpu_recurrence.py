@@ -1,11 +1,23 @@
 """The gated memory and the advantages (marl_amd.recurrence) against their 64-bit forms, elementwise, at bounds derived
 there: lengths from none to many tiles, odd widths, strided and expanded tensors, resets, values that must not be read,
 offsets beyond 32 bits, streams and HIP graphs."""
+import gc
+
 import pytest
 
 import seq_oracle as so
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def no_garbage():
+    """A HIP graph that the garbage collector frees while another one is captured ends the process (its destructor may not
+    run then): none is left from tests before, and none to tests after."""
+    gc.collect()
+    yield
+    gc.collect()
+
 
 SHAPES = [(1, 1, 1), (0, 3, 5), (3, 2, 64), (31, 3, 7), (32, 1, 65), (33, 2, 12), (100, 5, 61), (200, 64, 30),
           (9, 300, 256), (67, 280, 256), (40, 1100, 61), (1000, 2, 5), (4099, 1, 3), (700, 3, 256)]
@@ -241,7 +253,7 @@ def test_advantages_of_ring_slots_and_finished_episodes(torch_cuda):
     assert torch.equal(adv2[:10], adv[:10]) and torch.equal(ret2[:10], ret[:10])
 
 
-def test_captured_graphs_and_other_streams(torch_cuda):
+def test_captured_graphs_and_other_streams(torch_cuda, no_garbage):
     """Forward and backward in one HIP graph, replayed between eager work on other data; a second graph beside it; a side stream."""
     torch = torch_cuda
     from marl_amd.recurrence import advantages, gated_scan
@@ -284,7 +296,7 @@ def test_captured_graphs_and_other_streams(torch_cuda):
     assert all(torch.equal(a, b) for a, b in zip(other, work(*sets[0])))
 
 
-def test_capture_beside_a_live_eager_graph_is_refused(torch_cuda):
+def test_capture_beside_a_live_eager_graph_is_refused(torch_cuda, no_garbage):
     """The backward pass of such a capture would end the process: the call raises instead, before there is one."""
     torch = torch_cuda
     from marl_amd.policy_loss import clipped_policy_loss
