@@ -33,7 +33,7 @@
 // What bounds the phases of a workgroup (cycle stamps, hidden width 256, 192 features, 30 agents): layer 1 and the
 // prologue by the observation stream (every workgroup of the chip is in that phase at the same time); the hidden
 // layers by the matrix core plus the issue cost of the weight copies; the activations by their ~900 vector
-// instructions (256 accumulator reads, bias add and 0.01 product packed in pairs, 256 max, 128 packs).
+// instructions (256 accumulator reads, bias adds and 0.01 products, 256 max, 128 packs).
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -311,7 +311,7 @@ void k_policy_mlp(int n_a, int D, int K1, int A, int TPE, int ntiles, int half_f
                 const f32x4 b4 = bq[cur];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    // (bias add and the 0.01 product as packed pairs: v_pk_add_f32 / v_pk_mul_f32)
+                    // (bias add and the 0.01 product in pairs)
                     const f32x2 ta = f32x2{acc[u][m][4 * g], acc[u][m][4 * g + 1]} + f32x2{b4[0], b4[1]};
                     const f32x2 tb = f32x2{acc[u][m][4 * g + 2], acc[u][m][4 * g + 3]} + f32x2{b4[2], b4[3]};
                     const f32x2 sa = ta * 0.01f, sb = tb * 0.01f;
