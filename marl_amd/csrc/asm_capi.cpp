@@ -604,8 +604,8 @@ static int seq_dims(const char *fn, int dtype, int64_t T, int64_t B, int64_t D)
 {
     if (dtype != ASM_SEQ_F32 && dtype != ASM_SEQ_BF16) return fail(1, "%s: dtype = %d (supported: ASM_SEQ_F32, ASM_SEQ_BF16)", fn, dtype);
     if (T < 0 || B < 0 || D < 0) return fail(1, "%s: negative size", fn);
-    // (time steps and the threads of a launch are counted in 32 bits, offsets in 64)
-    if (T > (1 << 30) || B > (1 << 30) || D > (1 << 30) || B * D > (1 << 30))
+    // (time steps, channels or rows and the threads of a launch are counted in 32 bits, offsets in 64)
+    if (T > (1 << 30) || B > (1 << 29) || D > (1 << 29) || B * D > (1 << 29))
         return fail(1, "%s: T = %lld, B x D = %lld x %lld: too large", fn, (long long)T, (long long)B, (long long)D);
     return 0;
 }

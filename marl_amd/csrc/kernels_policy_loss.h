@@ -18,7 +18,7 @@
 constexpr int LOSS_SUMS = 5;                                            // gain, KL, entropy, cut rows, ratio; then A sums of ds
 
 struct LossDev {
-    int64_t rows, n, B;
+    uint32_t rows, n, B;
     int A;
     Rows mean, log_std, actions, old, ref, adv, mask;
     const float *moments;
@@ -41,15 +41,32 @@ template <int BS> __device__ __forceinline__ int64_t block_count(int64_t c, int6
     return t;
 }
 
-// Valid rows of each workgroup's share, for a mask and several workgroups.
-__global__ __launch_bounds__(256) void k_mask_count(int64_t rows, int64_t n, Rows mask, int64_t *counts)
+// Valid rows of each workgroup's share, for a mask and several workgroups.  LINEAR: one byte behind the other from a multiple
+// of 16 on, sixteen a load.
+__device__ __forceinline__ int nonzero_bytes(uint32_t w)
+{
+    w |= w >> 4; w |= w >> 2; w |= w >> 1;
+    return __popc(w & 0x01010101u);
+}
+template <bool LINEAR> __global__ __launch_bounds__(256) void k_mask_count(uint32_t rows, uint32_t n, Rows mask, int64_t *counts)
 {
     __shared__ int64_t sh[4];
     int64_t c = 0;
     const uint8_t *m = reinterpret_cast<const uint8_t *>(mask.p);
-    for (int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x; r < rows; r += (int64_t)gridDim.x * 256) {
-        const int64_t b = r / n, i = r - b * n;
-        c += m[b * mask.sb + i * mask.sn] != 0;
+    const uint32_t at = blockIdx.x * 256 + threadIdx.x, stride = gridDim.x * 256;
+    if (LINEAR) {
+        const uint4 *m4 = reinterpret_cast<const uint4 *>(m);
+        for (uint32_t k = at; k < rows / 16; k += stride) {
+            const uint4 w = m4[k];
+            c += nonzero_bytes(w.x) + nonzero_bytes(w.y) + nonzero_bytes(w.z) + nonzero_bytes(w.w);
+        }
+        const uint32_t r = rows / 16 * 16 + at;
+        if (r < rows) c += m[r] != 0;
+    } else {
+        for (uint32_t r = at; r < rows; r += stride) {
+            const uint32_t b = r / n, i = r - b * n;
+            c += m[(int64_t)b * mask.sb + (int64_t)i * mask.sn] != 0;
+        }
     }
     const int64_t t = block_count<256>(c, sh);
     if (threadIdx.x == 0) counts[blockIdx.x] = t;
@@ -128,7 +145,7 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
     if (masked) {
         int64_t c = 0;
         if (gridDim.x == 1) {
-            for (int64_t r = tid; r < p.rows; r += BS) { const int64_t b = r / p.n, i = r - b * p.n; c += maskp[b * p.mask.sb + i * p.mask.sn] != 0; }
+            for (uint32_t r = tid; r < p.rows; r += BS) { const uint32_t b = r / p.n, i = r - b * p.n; c += maskp[(int64_t)b * p.mask.sb + (int64_t)i * p.mask.sn] != 0; }
         } else {
             for (int k = tid; k < p.n_counts; k += BS) c += p.counts[k];
         }
@@ -144,10 +161,12 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
     for (int k = 0; k < LOSS_SUMS + AM; ++k) sum[k] = 0.0;
 
     // this workgroup's rows: [first, last)
-    const int64_t first = p.rows * blockIdx.x / gridDim.x, last = p.rows * (blockIdx.x + 1) / gridDim.x;
-    const int lane_row = tid / GL;
-    const int64_t db = ROWS / p.n, di = ROWS - db * p.n;                // (uniform)
-    int64_t b0 = (first + lane_row) / p.n, i = first + lane_row - b0 * p.n;
+    const uint32_t first = (uint32_t)((uint64_t)p.rows * blockIdx.x / gridDim.x), last = (uint32_t)((uint64_t)p.rows * (blockIdx.x + 1) / gridDim.x);
+    const uint32_t lane_row = tid / GL;
+    const uint32_t db = ROWS / p.n, di = ROWS - db * p.n;               // (uniform)
+    const uint32_t row0 = first + lane_row;
+    const int64_t b0 = row0 / p.n;
+    uint32_t i = row0 - (uint32_t)b0 * p.n;
     int64_t o_act = b0 * p.actions.sb + i * p.actions.sn + j0 * p.actions.sa;
     int64_t o_mean = 0, o_old = 0, o_ref = 0, o_adv = 0, o_mask = 0, o_std = 0;
     if (!LINEAR) {
@@ -155,16 +174,16 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
         o_adv = b0 * p.adv.sb + i * p.adv.sn; o_mask = b0 * p.mask.sb + i * p.mask.sn; o_std = b0 * p.log_std.sb + i * p.log_std.sn + j0 * p.log_std.sa;
     }
     struct Raw { Pack<TM, AM> mu, sd; float u[AM], old, ref, adv; uint8_t ok; };
-    auto fetch_row = [&](Raw &x, int64_t base) __attribute__((always_inline)) {       // base: the workgroup's row (uniform)
+    auto fetch_row = [&](Raw &x, uint32_t base) __attribute__((always_inline)) {       // base: the workgroup's row (uniform)
         if (LINEAR) {
-            const char *pm = reinterpret_cast<const char *>(p.mean.p) + base * (int64_t)(AM * GL * sizeof(TM));
+            const char *pm = reinterpret_cast<const char *>(p.mean.p) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM));
             x.mu = *reinterpret_cast<const Pack<TM, AM> *>(pm + (uint32_t)(tid * AM * sizeof(TM)));
-            if (!SHARED) x.sd = *reinterpret_cast<const Pack<TM, AM> *>(reinterpret_cast<const char *>(p.log_std.p) + base * (int64_t)(AM * GL * sizeof(TM)) + (uint32_t)(tid * AM * sizeof(TM)));
-            const uint32_t o = (uint32_t)lane_row * 4u;
-            x.old = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.old.p) + base * 4 + o);
-            if (own_ref) x.ref = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.ref.p) + base * 4 + o);
-            x.adv = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.adv.p) + base * 4 + o);
-            if (masked) x.ok = maskp[base + (uint32_t)lane_row];
+            if (!SHARED) x.sd = *reinterpret_cast<const Pack<TM, AM> *>(reinterpret_cast<const char *>(p.log_std.p) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM)) + (uint32_t)(tid * AM * sizeof(TM)));
+            const uint32_t o = lane_row * 4u;
+            x.old = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.old.p) + (int64_t)base * 4 + o);
+            if (own_ref) x.ref = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.ref.p) + (int64_t)base * 4 + o);
+            x.adv = *reinterpret_cast<const float *>(reinterpret_cast<const char *>(p.adv.p) + (int64_t)base * 4 + o);
+            if (masked) x.ok = (maskp + base)[lane_row];
         } else {
 #pragma unroll
             for (int j = 0; j < AM; ++j)
@@ -185,7 +204,7 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
         i += di;
         const bool nb = i >= p.n;
         if (nb) i -= p.n;
-        auto move = [&](int64_t &o, const Rows &t) __attribute__((always_inline)) { o += db * t.sb + di * t.sn; if (nb) o += t.sb - p.n * t.sn; };
+        auto move = [&](int64_t &o, const Rows &t) __attribute__((always_inline)) { o += (int64_t)db * t.sb + (int64_t)di * t.sn; if (nb) o += t.sb - (int64_t)p.n * t.sn; };
         move(o_act, p.actions);
         if (!LINEAR) {
             move(o_mean, p.mean); move(o_old, p.old); move(o_adv, p.adv);
@@ -196,7 +215,7 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
     };
     Raw cur, nxt;
     if (first + lane_row < last) fetch_row(cur, first);
-    for (int64_t base = first; base < last; base += ROWS) {
+    for (uint32_t base = first; base < last; base += ROWS) {
         // (the GL lanes of a row go the same way)
         const bool have = base + lane_row < last;
         if (base + ROWS + lane_row < last) { move_on(); fetch_row(nxt, base + ROWS); }
@@ -249,11 +268,11 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
         }
         if (have) {
             if (LINEAR) {
-                char *pd = reinterpret_cast<char *>(p.dmean) + base * (int64_t)(AM * GL * sizeof(TM));
+                char *pd = reinterpret_cast<char *>(p.dmean) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM));
                 put<TM, AM>(pd, 0, (uint32_t)(tid * AM * sizeof(TM)), dm);
-                if (!SHARED) put<TM, AM>(reinterpret_cast<char *>(p.dstd) + base * (int64_t)(AM * GL * sizeof(TM)), 0, (uint32_t)(tid * AM * sizeof(TM)), ds);
+                if (!SHARED) put<TM, AM>(reinterpret_cast<char *>(p.dstd) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM)), 0, (uint32_t)(tid * AM * sizeof(TM)), ds);
             } else {
-                const int64_t at = (base + lane_row) * p.A + j0;
+                const int64_t at = (int64_t)(base + lane_row) * p.A + j0;
 #pragma unroll
                 for (int j = 0; j < AM; ++j)
                     if (j0 + j < p.A) {
@@ -326,14 +345,14 @@ template <typename TM> __global__ __launch_bounds__(256) void k_policy_loss_scal
     }
 }
 
-struct ActDev { int64_t rows, n; int A, shared; Rows mean, log_std, noise, actions, log_pi; };
+struct ActDev { uint32_t rows, n; int A; Rows mean, log_std, noise, actions, log_pi; };
 
 // u = mu + e^s noise (or the given u), and the log-probability of u as it is stored.
 template <typename TM, bool DRAW> __global__ __launch_bounds__(256) void k_gaussian_act(ActDev p)
 {
-    const int64_t r = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const uint32_t r = blockIdx.x * 256 + threadIdx.x;
     if (r >= p.rows) return;
-    const int64_t b = r / p.n, i = r - b * p.n;
+    const int64_t b = r / p.n, i = r - (uint32_t)b * p.n;
     const TM *mean = reinterpret_cast<const TM *>(p.mean.p) + b * p.mean.sb + i * p.mean.sn;
     const TM *std_ = reinterpret_cast<const TM *>(p.log_std.p) + b * p.log_std.sb + i * p.log_std.sn;
     const float *noise = DRAW ? reinterpret_cast<const float *>(p.noise.p) + b * p.noise.sb + i * p.noise.sn : nullptr;

@@ -535,12 +535,12 @@ __global__ __launch_bounds__(256) void k_moments(const double *mom, int64_t n, f
 
 // One step of the memory: state <- a k state + (1 - a) x, out = the new state in the inputs' type.
 template <typename T, int V>
-__global__ __launch_bounds__(256) void k_scan_step(int64_t n, int64_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb,
+__global__ __launch_bounds__(256) void k_scan_step(uint32_t n, uint32_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb,
                                                    float *state, const uint8_t *reset, int64_t r_sb, void *out, int64_t o_sb)
 {
-    const int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
+    const uint32_t e = (blockIdx.x * 256 + threadIdx.x) * V;
     if (e >= n) return;
-    const int64_t b = e / D, d = e - b * D;
+    const int64_t b = e / D, d = e - (uint32_t)b * D;
     float g[V], xv[V], s[V];
     load_vec<T, V>(g, gate, b * g_sb + d);
     load_vec<T, V>(xv, x, b * x_sb + d);

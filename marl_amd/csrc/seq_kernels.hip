@@ -151,7 +151,7 @@ int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t 
     const size_t e = dtype ? 2 : 4;
     const bool vec = D % 4 == 0 && vec_ok(gate, 0, g_sb, e, 4) && vec_ok(x, 0, x_sb, e, 4) && vec_ok(out, 0, o_sb, e, 4) && aligned(state, 16);
     const unsigned grid = (unsigned)((n / (vec ? 4 : 1) + 255) / 256);
-#define GO(T, V) hipLaunchKernelGGL((k_scan_step<T, V>), dim3(grid), dim3(256), 0, st, n, D, gate, g_sb, x, x_sb, state, reset, r_sb, out, o_sb)
+#define GO(T, V) hipLaunchKernelGGL((k_scan_step<T, V>), dim3(grid), dim3(256), 0, st, (uint32_t)n, (uint32_t)D, gate, g_sb, x, x_sb, state, reset, r_sb, out, o_sb)
     if (dtype == 0) { if (vec) GO(float, 4); else GO(float, 1); }
     else { if (vec) GO(bf16, 4); else GO(bf16, 1); }
 #undef GO
@@ -222,7 +222,10 @@ template <typename TM, int AM, int GL, bool SHARED, bool LINEAR> static int loss
     const int groups = loss_groups(p.rows, p.A);
     if (p.mask.p) {
         p.n_counts = COUNT_GROUPS;
-        hipLaunchKernelGGL(k_mask_count, dim3(COUNT_GROUPS), dim3(256), 0, st, p.rows, p.n, p.mask, const_cast<int64_t *>(p.counts));
+        const bool linear = (p.mask.sn == 1 || p.n == 1) && (p.mask.sb == p.n || p.B == 1) && aligned(p.mask.p, 16);
+        int64_t *counts = const_cast<int64_t *>(p.counts);
+        if (linear) hipLaunchKernelGGL(k_mask_count<true>, dim3(COUNT_GROUPS), dim3(256), 0, st, p.rows, p.n, p.mask, counts);
+        else hipLaunchKernelGGL(k_mask_count<false>, dim3(COUNT_GROUPS), dim3(256), 0, st, p.rows, p.n, p.mask, counts);
         LAUNCH_CHECK();
     }
     hipLaunchKernelGGL((k_policy_loss<TM, AM, GL, SHARED, LINEAR, 256>), dim3(groups), dim3(256), 0, st, p);
@@ -234,7 +237,7 @@ template <typename TM, int AM, int GL, bool SHARED, bool LINEAR> static int loss
 template <typename TM, int AM, int GL> static int loss_pick(const LossDev &p, bool shared, hipStream_t st)
 {
     const size_t row = sizeof(TM) * AM;
-    const auto in_line = [&](const Rows &t, int A, size_t align) { return !t.p || ((A == 1 || t.sa == 1) && (t.sn == A || p.n == 1) && (t.sb == p.n * A || p.B == 1) && aligned(t.p, align)); };
+    const auto in_line = [&](const Rows &t, int A, size_t align) { return !t.p || ((A == 1 || t.sa == 1) && (t.sn == A || p.n == 1) && (t.sb == (int64_t)p.n * A || p.B == 1) && aligned(t.p, align)); };
     const bool linear = p.A == AM * GL && in_line(p.mean, p.A, row) && (shared || in_line(p.log_std, p.A, row)) && in_line(p.old, 1, 4) && in_line(p.ref, 1, 4) &&
                         in_line(p.adv, 1, 4) && in_line(p.mask, 1, 1) && aligned(p.dmean, row) && (shared || aligned(p.dstd, row));
     if (linear) return shared ? loss_go<TM, AM, GL, true, true>(p, st) : loss_go<TM, AM, GL, false, true>(p, st);
@@ -253,7 +256,7 @@ template <typename TM> static int loss_width(const LossDev &p, bool shared, hipS
 int launch_policy_loss(const LossArgs &a, hipStream_t st)
 {
     LossDev p{};
-    p.rows = a.B * a.n; p.n = std::max<int64_t>(a.n, 1); p.B = a.B; p.A = a.A;
+    p.rows = (uint32_t)(a.B * a.n); p.n = (uint32_t)std::max<int64_t>(a.n, 1); p.B = (uint32_t)a.B; p.A = a.A;
     p.mean = a.mean; p.log_std = a.log_std; p.actions = a.actions; p.old = a.log_pi_old;
     p.ref = a.log_pi_ref.p ? a.log_pi_ref : a.log_pi_old;
     p.adv = a.adv; p.mask = a.mask; p.moments = a.adv_moments;
@@ -282,7 +285,7 @@ int launch_gaussian_act(const ActArgs &a, hipStream_t st)
 {
     const int64_t rows = a.B * a.n;
     if (rows == 0) return 0;
-    const ActDev p{rows, a.n, a.A, 0, a.mean, a.log_std, a.noise, a.actions, a.log_pi};
+    const ActDev p{(uint32_t)rows, (uint32_t)a.n, a.A, a.mean, a.log_std, a.noise, a.actions, a.log_pi};
     const unsigned grid = (unsigned)((rows + 255) / 256);
     if (a.dtype == 0) {
         if (a.noise.p) hipLaunchKernelGGL((k_gaussian_act<float, true>), dim3(grid), dim3(256), 0, st, p);

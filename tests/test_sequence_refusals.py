@@ -117,7 +117,7 @@ def test_c_abi_refuses_before_it_launches():
     p = 1 << 20
     fwd = lambda dt=0, T=T, B=B, D=D, gate=p, x=p, h=p, ws=None, n=0: lib.asm_gated_scan_forward(  # noqa: E731
         dt, T, B, D, gate, 0, 0, x, 0, 0, None, None, 0, 0, None, h, 0, 0, None, ws, n, None)
-    for kw, msg in ((dict(dt=7), "dtype"), (dict(T=-1), "negative"), (dict(B=1 << 31), "too large"), (dict(B=1 << 20, D=1 << 20), "too large"),
+    for kw, msg in ((dict(dt=7), "dtype"), (dict(T=-1), "negative"), (dict(B=1 << 31), "too large"), (dict(B=1 << 29, D=2), "too large"), (dict(B=1 << 20, D=1 << 20), "too large"),
                     (dict(T=1 << 31), "too large"), (dict(gate=None), "NULL"), (dict(x=None), "NULL"), (dict(h=None), "NULL"),
                     (dict(T=100000), "workspace"), (dict(T=100000, ws=p, n=8), "workspace"), (dict(T=100000, ws=p + 8, n=1 << 40), "aligned")):
         assert fwd(**kw) != 0 and msg in _msg(lib), (kw, _msg(lib))
