@@ -39,29 +39,35 @@ struct Plan { int V, NW, L, nsplit, Ts; };
 //   491520            706 / 401                    695 / 359                    676 / 325
 // Many channels fill the chip by themselves, and a wave that shares nothing waits for nobody: from 600 KB a time step on.  Below,
 // four waves side by side in time; from 49152 channels on two of them in a lane (half the address work).  Rows that are not aligned to two or four
-// values go one channel a lane.  Fewer than 256 workgroups and ten tiles of time or more: the time axis is cut until there are 512,
-// down to one tile a stretch (20011 steps x 183 channels, forward + backward: 61 stretches 97 us, 157 stretches 61 us; 1920 channels
-// forward, cut / whole: 256 steps 7.8 / 8.4 us, 192 steps 7.7 / 7.1 us, and a launch less on the host).
-Plan scan_plan(int64_t T, int64_t C, size_t size, bool vec2, bool vec4)
+// values go one channel a lane.
+// Fewer than 256 workgroups of one channel a lane: what counts is how often a tile's loads are waited for.  Up to `whole` steps eight
+// waves share a tile and one launch does it all; from there on the time axis is cut until there are 512 workgroups, down to one tile
+// a stretch (1920 channels, forward + backward, us: 100 steps eight waves 13, four 14, cut 15; 200 steps 19, 22, 16; 333 steps
+// 24, 31, 19; 2000 steps 95, 144, 39; on the host each of the two launches more costs 4 us or, in a backward pass, up to 20.
+// 20011 steps x 183 channels: 61 stretches 97 us, 157 stretches 58 us).
+Plan scan_plan(int64_t T, int64_t C, size_t size, bool vec2, bool vec4, int64_t whole = 320)
 {
     Plan p{1, 4, 8, 1, 0};
     if (vec4 && C * (int64_t)size >= 600000) p = {4, 1, 4, 1, 0};
     else if (vec2 && C >= 49152) p = {2, 4, 4, 1, 0};
-    const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V), tile = p.NW * p.L, tiles = std::max<int64_t>(1, (T + tile - 1) / tile);
+    const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V);
+    const bool few = p.V == 1 && groups < 256;
+    if (few && T < whole) p.NW = 8;
+    const int64_t tile = p.NW * p.L, tiles = std::max<int64_t>(1, (T + tile - 1) / tile);
     int64_t want = 1;
-    if (p.V == 1 && groups < 256 && tiles >= 10) want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / groups, tiles), 256));
+    if (few && T >= whole) want = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / groups, tiles), 256));
     const int64_t per = (tiles + want - 1) / want;
     p.Ts = (int)(per * tile);
     p.nsplit = (int)((tiles + per - 1) / per);
     return p;
 }
 // (the workspace of any alignment)
-int most_splits(int64_t T, int64_t C, size_t size) { return scan_plan(T, C, size, false, false).nsplit; }
+int most_splits(int64_t T, int64_t C, size_t size, int64_t whole = 320) { return scan_plan(T, C, size, false, false, whole).nsplit; }
 
 template <int V, int NW, int L, class O> int scan_go(const O &op, const ScanGeom &q, double *mom, hipStream_t st)
 {
     const unsigned groups = (unsigned)((q.C + 64 * V - 1) / (64 * V));
-    if constexpr (V == 1)
+    if constexpr (V == 1 && NW == 4)
         if (q.nsplit > 1) {
             hipLaunchKernelGGL((k_scan<O, V, NW, L, true>), dim3(groups, q.nsplit - 1), dim3(64 * NW), 0, st, op, q, (double *)nullptr);
             LAUNCH_CHECK();
@@ -75,10 +81,10 @@ int scan_typed(const Plan &p, bool far, const ScanGeom &q, Fill fill, hipStream_
 {
     if (p.V == 4) { Op<T, 4, MSK, uint32_t> op; fill(op); return scan_go<4, 1, 4>(op, q, nullptr, st); }
     if (p.V == 2) { Op<T, 2, MSK, uint32_t> op; fill(op); return scan_go<2, 4, 4>(op, q, nullptr, st); }
-    if (far) { Op<T, 1, MSK, int64_t> op; fill(op); return scan_go<1, 4, 8>(op, q, nullptr, st); }
+    if (far) { Op<T, 1, MSK, int64_t> op; fill(op); return p.NW == 8 ? scan_go<1, 8, 8>(op, q, nullptr, st) : scan_go<1, 4, 8>(op, q, nullptr, st); }
     Op<T, 1, MSK, uint32_t> op;
     fill(op);
-    return scan_go<1, 4, 8>(op, q, nullptr, st);
+    return p.NW == 8 ? scan_go<1, 8, 8>(op, q, nullptr, st) : scan_go<1, 4, 8>(op, q, nullptr, st);
 }
 template <template <typename, int, bool, typename> class Op, class Fill>
 int scan_dispatch(int dtype, bool msk, const Plan &p, bool far, const ScanGeom &q, Fill fill, hipStream_t st)
@@ -159,10 +165,12 @@ int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t 
     return 0;
 }
 
+constexpr int64_t ADV_WHOLE = 160;                                      // (91 channels, whole / cut, us: 96 steps 7.1 / 8.2, 192 steps 8.8 / 8.3, 333 steps 14 / 8.5)
+
 // The stretches' compositions, then three doubles a workgroup.
 int64_t advantages_workspace(int64_t T, int64_t C)
 {
-    const int n = most_splits(T, C, 4);
+    const int n = most_splits(T, C, 4, ADV_WHOLE);
     return (n > 1 ? (int64_t)n * 2 * C * 4 + 16 : 0) + (C + 63) / 64 * n * 24;
 }
 
@@ -188,12 +196,12 @@ int launch_advantages(const AdvArgs &a, hipStream_t st)
         return a.C % V == 0 && vec_ok(a.rewards, a.rew_st, 0, 4, V) && vec_ok(a.values, a.val_st, 0, 4, V) && vec_ok(a.dones, a.done_st, 0, 1, V) &&
                aligned(a.adv, 4 * V) && aligned(a.ret, 4 * V);
     };
-    Plan p = scan_plan(a.T, a.C, 4, false, false);
+    Plan p = scan_plan(a.T, a.C, 4, false, false, ADV_WHOLE);
     if (rows(4) && a.C >= 49152) p = {4, 4, 4, 1, (int)((a.T + 15) / 16 * 16)};        // (200 x 122880: 75 us; two channels a lane 80 us, one wave for all of time 82 us)
     const bool msk = a.dones || a.lengths, mom = a.moments != nullptr;
 #define GO(V, NW, L) (msk ? (mom ? advantages_go<V, NW, L, true, true>(a, p, st) : advantages_go<V, NW, L, true, false>(a, p, st)) \
                           : (mom ? advantages_go<V, NW, L, false, true>(a, p, st) : advantages_go<V, NW, L, false, false>(a, p, st)))
-    return p.V == 4 ? GO(4, 4, 4) : GO(1, 4, 8);
+    return p.V == 4 ? GO(4, 4, 4) : p.NW == 8 ? GO(1, 8, 8) : GO(1, 4, 8);
 #undef GO
 }
 

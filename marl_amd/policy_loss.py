@@ -14,7 +14,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .recurrence import _DTYPES, _FLAGS, _call, _guard_leaves, _need, _on_device, _ptr, _workspace
+from .recurrence import _DTYPES, _FLAGS, _call, _guard_leaves, _need, _on_device, _once, _ptr, _workspace
 
 STATS_FIELDS = ("gain", "kl", "entropy", "clipped", "ratio", "rows")
 _NO_ROWS = (0, 0, 0, 0)
@@ -104,11 +104,11 @@ class _ClippedLoss(torch.autograd.Function):
         return loss, stats
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, g, _):
         none = (None,) * 10
         if g is None:
             return (None, None) + none
+        _once("clipped_policy_loss")
         # the gradients of the forward pass are handed out once; a second backward pass over a retained graph makes its own
         tensors = ctx.saved_tensors                                     # (notices inputs overwritten since)
         grads, ctx.grads = ctx.grads, None
@@ -180,7 +180,6 @@ def _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv
     raise ValueError(f"{fn}: bad arguments")
 
 
-@torch.no_grad()
 def gaussian_act(mean: torch.Tensor, log_std: torch.Tensor, noise: torch.Tensor, *, actions: Optional[torch.Tensor] = None,
                  log_pi: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """A rollout's actions, without gradients: (actions, log_pi) with actions = mean + e^log_std noise and log_pi the
@@ -190,7 +189,6 @@ def gaussian_act(mean: torch.Tensor, log_std: torch.Tensor, noise: torch.Tensor,
     return _act("gaussian_act", mean, log_std, noise, actions, log_pi)
 
 
-@torch.no_grad()
 def gaussian_log_pi(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Tensor, *, log_pi: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Log-probabilities of given actions, without gradients: what a reference policy says of a recorded episode."""
     return _act("gaussian_log_pi", mean, log_std, None, actions, log_pi)[1]

@@ -65,6 +65,12 @@ def _call(name: str, dev: torch.device, *args) -> None:
         _lib.check(rc, name)
 
 
+def _once(fn: str) -> None:
+    """(what torch.autograd.function.once_differentiable makes sure of, at a twentieth of its price a call)"""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{fn} is differentiable once: no create_graph=True through it")
+
+
 def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
     """A leaf's accumulation node belongs to the stream it was first used on and lives as long as any graph that uses the
     leaf; a backward pass captured into a HIP graph would have to join that other stream, which ends the process.
@@ -111,8 +117,8 @@ class _GatedScan(torch.autograd.Function):
         return h, last
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dlast):
+        _once("gated_scan")
         gate, x, h, h0, resets, lengths = ctx.saved_tensors
         T, B, D = ctx.dims
         bf, dev, dt = ctx.batch_first, gate.device, _DTYPES[gate.dtype]
@@ -196,7 +202,6 @@ def _time_rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.is_contiguous() or t[0].is_contiguous() else t.contiguous()
 
 
-@torch.no_grad()
 def advantages(rewards: torch.Tensor, values: torch.Tensor, *, dones: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
                gamma: float = 0.95, lam: float = 0.95, moments: bool = False):
     """Advantages and returns of an episode, without gradients: (adv, ret), or (adv, ret, moments).

@@ -332,3 +332,15 @@ def test_backward_notices_inputs_overwritten_since(torch_cuda):
     want = so.scan(gate, x, dlast=torch.ones(2, 8))
     so.within(gate.grad, *want["dgate"], "gate")
     so.within(x.grad, *want["dx"], "x")
+
+
+def test_second_derivatives_are_refused(torch_cuda):
+    torch = torch_cuda
+    from marl_amd.policy_loss import clipped_policy_loss
+    from marl_amd.recurrence import gated_scan
+    gate, x = (torch.randn(4, 2, 8, device="cuda", requires_grad=True) for _ in range(2))
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(gated_scan(gate, x)[0].sum(), gate, create_graph=True)
+    mean, row = torch.randn(6, 2, device="cuda", requires_grad=True), torch.randn(6, device="cuda")
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(clipped_policy_loss(mean, torch.zeros(2, device="cuda"), mean.detach(), row, row)[0], mean, create_graph=True)
