@@ -375,12 +375,15 @@ int asm_policy_mlp_act_bf16(int E, int n_a, int obs_dim, int hidden, int act_dim
  * in float32; h_t is rounded once to dtype where it is stored.  resets (nullable; element (t, b) at [t * r_st + b * r_sb]):
  * where nonzero, the state in front of step t counts as zero, whatever it holds.  lengths (nullable, [B], clamped to
  * 0..T): steps from lengths[b] on are not part of the sequence: h is zero there, the state passes.  h_last
- * (nullable): [B][D], the state behind the last step.  h0, h_last, dh0, dh_last: [B][D] contiguous. */
+ * (nullable): [B][D], the state behind the last step.  h0, h_last, dh0, dh_last: [B][D] contiguous.
+ * kept (nullable): asm_gated_scan_kept bytes (aligned to 16) in which the forward pass leaves the states in front of every eighth
+ * step for the backward pass of the same arguments, which then reads those and not h: where that function returns 0, pass NULL. */
+int64_t asm_gated_scan_kept(int dtype, int64_t T, int64_t B, int64_t D);
 int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D);
 int asm_gated_scan_forward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
                            const void *x, int64_t x_st, int64_t x_sb, const float *h0 /*nullable*/, const uint8_t *resets /*nullable*/,
                            int64_t r_st, int64_t r_sb, const int32_t *lengths /*nullable*/, void *h, int64_t h_st, int64_t h_sb,
-                           float *h_last /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
+                           float *h_last /*nullable*/, float *kept /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
 /* Gradients of the above: dh (nullable: zeros) of h, dh_last (nullable: zeros) of h_last.  h: the forward pass's output.
  * Writes dgate, dx (zero beyond a sequence's length) and dh0 (nullable). */
 int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
@@ -388,7 +391,8 @@ int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const vo
                             const float *h0 /*nullable*/, const uint8_t *resets /*nullable*/, int64_t r_st, int64_t r_sb,
                             const int32_t *lengths /*nullable*/, const void *dh /*nullable*/, int64_t dh_st, int64_t dh_sb,
                             const float *dh_last /*nullable*/, void *dgate, int64_t dgate_st, int64_t dgate_sb, void *dx,
-                            int64_t dx_st, int64_t dx_sb, float *dh0 /*nullable*/, void *ws, int64_t ws_bytes, void *stream);
+                            int64_t dx_st, int64_t dx_sb, float *dh0 /*nullable*/, const float *kept /*nullable*/, void *ws, int64_t ws_bytes,
+                            void *stream);
 /* One step of a rollout: state [B][D] float32 is updated in place, out gets the new state in dtype.  Row b of gate, x and
  * out starts at b * *_sb; reset (nullable): element b at [b * r_sb], nonzero: the state counts as zero first. */
 int asm_gated_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t gate_sb, const void *x, int64_t x_sb,

@@ -51,7 +51,7 @@ EXPORTS = ["_get_observation", "_get_reward", "_sf_b2b_all", "_get_dist_b2w", "c
            "asm_debug_sqrt_f64", "asm_debug_cos_f32_max_err", "asm_get_observation_noalloc", "asm_lattice_build",
            "asm_batch_check_lattice", "asm_set_step_schedule", "asm_debug_step_schedule",
            "asm_policy_mlp_forward_bf16", "asm_policy_mlp_act_bf16", "asm_obs_rows_f32",
-           "asm_gated_scan_workspace", "asm_gated_scan_forward", "asm_gated_scan_backward", "asm_gated_scan_step",
+           "asm_gated_scan_workspace", "asm_gated_scan_kept", "asm_gated_scan_forward", "asm_gated_scan_backward", "asm_gated_scan_step",
            "asm_advantages_workspace", "asm_advantages_f32", "asm_policy_loss_workspace", "asm_policy_loss",
            "asm_policy_loss_scale", "asm_gaussian_act"]
 
@@ -119,11 +119,13 @@ def load() -> C.CDLL:
     f32, f64 = C.c_float, C.c_double
     lib.asm_gated_scan_workspace.restype = i64
     lib.asm_gated_scan_workspace.argtypes = [i32, i64, i64, i64]
+    lib.asm_gated_scan_kept.restype = i64
+    lib.asm_gated_scan_kept.argtypes = [i32, i64, i64, i64]
     lib.asm_gated_scan_forward.restype = C.c_int
-    lib.asm_gated_scan_forward.argtypes = [i32, i64, i64, i64] + [vp, i64, i64] * 2 + [vp, vp, i64, i64, vp] + [vp, i64, i64] + [vp, vp, i64, vp]
+    lib.asm_gated_scan_forward.argtypes = [i32, i64, i64, i64] + [vp, i64, i64] * 2 + [vp, vp, i64, i64, vp] + [vp, i64, i64] + [vp, vp, vp, i64, vp]
     lib.asm_gated_scan_backward.restype = C.c_int
     lib.asm_gated_scan_backward.argtypes = [i32, i64, i64, i64] + [vp, i64, i64] * 3 + [vp, vp, i64, i64, vp] + [vp, i64, i64] + [vp] + \
-        [vp, i64, i64] * 2 + [vp, vp, i64, vp]
+        [vp, i64, i64] * 2 + [vp, vp, vp, i64, vp]
     lib.asm_gated_scan_step.restype = C.c_int
     lib.asm_gated_scan_step.argtypes = [i32, i64, i64, vp, i64, vp, i64, vp, vp, i64, vp, i64, vp]
     lib.asm_advantages_workspace.restype = i64

@@ -622,20 +622,27 @@ int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
     return B * D == 0 ? 0 : asmseq::scan_workspace(dtype, T, B, D);
 }
 
+int64_t asm_gated_scan_kept(int dtype, int64_t T, int64_t B, int64_t D)
+{
+    if (seq_dims("asm_gated_scan_kept", dtype, T, B, D)) return -1;
+    return B * D == 0 || T == 0 ? 0 : asmseq::scan_kept(dtype, T, B, D);
+}
+
 int asm_gated_scan_forward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,
                            const void *x, int64_t x_st, int64_t x_sb, const float *h0, const uint8_t *resets, int64_t r_st,
-                           int64_t r_sb, const int32_t *lengths, void *h, int64_t h_st, int64_t h_sb, float *h_last, void *ws,
-                           int64_t ws_bytes, void *stream)
+                           int64_t r_sb, const int32_t *lengths, void *h, int64_t h_st, int64_t h_sb, float *h_last, float *kept,
+                           void *ws, int64_t ws_bytes, void *stream)
 {
     if (int rc = seq_dims("asm_gated_scan_forward", dtype, T, B, D)) return rc;
     if (B * D == 0) return 0;
     if (T > 0 && (!gate || !x || !h)) return fail(1, "asm_gated_scan_forward: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(kept) & 15) return fail(1, "asm_gated_scan_forward: kept is not aligned to 16 bytes");
     if (int rc = seq_ws("asm_gated_scan_forward", ws, ws_bytes, asmseq::scan_workspace(dtype, T, B, D))) return rc;
     asmseq::ScanArgs a{};
     a.dtype = dtype; a.T = T; a.B = B; a.D = D;
     a.gate = {gate, gate_st, gate_sb}; a.x = {x, x_st, x_sb}; a.h0 = h0;
     a.resets = resets; a.r_st = r_st; a.r_sb = r_sb; a.lengths = lengths;
-    a.out = {h, h_st, h_sb}; a.h_last = h_last; a.ws = ws;
+    a.out = {h, h_st, h_sb}; a.h_last = h_last; a.kept = kept; a.ws = ws;
     int rc = asmseq::launch_scan_forward(a, (hipStream_t)stream);
     return rc ? hip_fail(rc, "asm_gated_scan_forward") : 0;
 }
@@ -644,18 +651,19 @@ int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const vo
                             const void *x, int64_t x_st, int64_t x_sb, const void *h, int64_t h_st, int64_t h_sb,
                             const float *h0, const uint8_t *resets, int64_t r_st, int64_t r_sb, const int32_t *lengths,
                             const void *dh, int64_t dh_st, int64_t dh_sb, const float *dh_last, void *dgate, int64_t dgate_st,
-                            int64_t dgate_sb, void *dx, int64_t dx_st, int64_t dx_sb, float *dh0, void *ws, int64_t ws_bytes,
-                            void *stream)
+                            int64_t dgate_sb, void *dx, int64_t dx_st, int64_t dx_sb, float *dh0, const float *kept, void *ws,
+                            int64_t ws_bytes, void *stream)
 {
     if (int rc = seq_dims("asm_gated_scan_backward", dtype, T, B, D)) return rc;
     if (B * D == 0) return 0;
     if (T > 0 && (!gate || !x || !h || !dgate || !dx)) return fail(1, "asm_gated_scan_backward: NULL pointer");
+    if (reinterpret_cast<uintptr_t>(kept) & 15) return fail(1, "asm_gated_scan_backward: kept is not aligned to 16 bytes");
     if (int rc = seq_ws("asm_gated_scan_backward", ws, ws_bytes, asmseq::scan_workspace(dtype, T, B, D))) return rc;
     asmseq::ScanArgs a{};
     a.dtype = dtype; a.T = T; a.B = B; a.D = D;
     a.gate = {gate, gate_st, gate_sb}; a.x = {x, x_st, x_sb}; a.h = {h, h_st, h_sb}; a.dh = {dh, dh_st, dh_sb};
     a.h0 = h0; a.dh_last = dh_last; a.resets = resets; a.r_st = r_st; a.r_sb = r_sb; a.lengths = lengths;
-    a.dgate = {dgate, dgate_st, dgate_sb}; a.dx = {dx, dx_st, dx_sb}; a.dh0 = dh0; a.ws = ws;
+    a.dgate = {dgate, dgate_st, dgate_sb}; a.dx = {dx, dx_st, dx_sb}; a.dh0 = dh0; a.kept = const_cast<float *>(kept); a.ws = ws;
     int rc = asmseq::launch_scan_backward(a, (hipStream_t)stream);
     return rc ? hip_fail(rc, "asm_gated_scan_backward") : 0;
 }

@@ -122,11 +122,12 @@ template <typename T, int V, typename OFF> __device__ __forceinline__ void put(c
 // is written).
 
 template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
-    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false, CUTS = MSK;
+    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = true;
     Seq gate, x;
     SeqOut out;
     const float *h0;
     float *h_last;
+    float *ck;                                                          // the state in front of every eighth step, [T / 8][C] (nullable)
     Marks marks;
     struct Lane { const char *g, *x, *o, *r; OFF og, ox, oo; MarkLane<OFF> m; };
     struct Raw { Words<T, V> g, x; Words<uint8_t, 1> cut; };
@@ -178,7 +179,7 @@ template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
 };
 
 template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
-    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false, CUTS = MSK;
+    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = false;
     Seq gate, x, h, dh;
     SeqOut dgate, dx;
     const float *h0, *dh_last;
@@ -258,7 +259,7 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
 
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.
 template <int V, bool MSK, bool MOM> struct AdvantageOp {
-    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK;
+    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK, KEEPS = false;
     const float *rewards, *values;
     int64_t rew_st, val_st, done_st;
     const uint8_t *dones;
@@ -470,6 +471,9 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
                 CA[v] = joined<CUTS>(A, CA[v]);
             }
         }
+        if constexpr (!AGG && NW == 1 && Op::KEEPS) {
+            if (op.ck && have && u0 % 8 == 0) store_vec<float, V>(op.ck, (int64_t)(u0 / 8) * q.C + w.ch, c);
+        }
         if (!AGG) {
 #pragma unroll
             for (int l = 0; l < L; ++l) {
@@ -508,6 +512,84 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
             mom[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 3 + threadIdx.x] = t;
         }
     }
+}
+
+// The backward pass of many channels, one wave for all of time, from the states that the forward pass kept in front of every eighth step:
+// the eight states in between are computed again, in float32, from the gates and inputs the pass reads anyway, so it reads
+// gate, x, dh and an eighth of a state instead of gate, x, dh and h (200 x 1920 x 256 float32: 5.25 arrays in and out for 6).
+template <typename T, int V, bool MSK>
+__global__ __launch_bounds__(64) void k_scan_back_kept(BackwardOp<T, V, MSK, uint32_t> op, ScanGeom q, const float *ck)
+{
+    constexpr int L = 8;
+    typedef BackwardOp<T, V, MSK, uint32_t> Op;
+    const uint32_t first = blockIdx.x * 64u * V, mine_ch = first + threadIdx.x * V;
+    const bool have = mine_ch < q.C;
+    Place w;
+    w.ch = have ? mine_ch : first;
+    w.b0 = __builtin_amdgcn_readfirstlane(first / q.D);
+    const uint32_t rel = w.ch - w.b0 * q.D;
+    w.db = rel / q.D;
+    w.d = rel - w.db * q.D;
+    const typename Op::Lane ln = op.lane(q, w);
+    struct Raw { Words<T, V> g, x, dh; Words<uint8_t, 1> cut; };
+    Raw raw[L];
+    float state[V], c[V];
+    auto load = [&](auto clamp, int t0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const Step s = decltype(clamp)::value ? Step{t0 + l < q.T ? t0 + l : q.T - 1, 0} : Step{t0, l};
+            fetch(raw[l].g, ln.g, step_off(s, op.gate.st), ln.og);
+            fetch(raw[l].x, ln.x, step_off(s, op.x.st), ln.ox);
+            if (op.dh.p) fetch(raw[l].dh, ln.dh, step_off(s, op.dh.st), ln.odh);
+            if (MSK) { raw[l].cut.w = 0; if (op.marks.resets) fetch(raw[l].cut, ln.r, step_off(s, op.marks.r_st), ln.m.r); }
+        }
+        load_vec<float, V>(state, ck, (int64_t)(t0 / L) * q.C + w.ch);
+    };
+    op.carry0(c, w.ch);
+    auto work = [&](auto full, auto next, int t0) __attribute__((always_inline)) {
+        constexpr bool FULL = decltype(full)::value, NEXT = decltype(next)::value;
+        float a[L][V], b[L][V], m[L][V], dh[L][V], h[V];
+        bool cut[L];
+#pragma unroll
+        for (int v = 0; v < V; ++v) h[v] = state[v];
+#pragma unroll
+        for (int l = 0; l < L; ++l) {
+            const bool on = (FULL || t0 + l < q.T) && (!MSK || t0 + l < ln.m.len);
+            cut[l] = MSK && raw[l].cut.get(0);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                gate_pair(raw[l].g.get(v), a[l][v], b[l][v]);
+                const float before = cut[l] ? 0.f : h[v], x = raw[l].x.get(v);
+                m[l][v] = (before - x) * a[l][v];
+                dh[l][v] = op.dh.p ? raw[l].dh.get(v) : 0.f;
+                const float after = __fmaf_rn(a[l][v], before, b[l][v] * x);
+                h[v] = on ? after : h[v];
+            }
+        }
+        if constexpr (NEXT) load(std::false_type{}, t0 - L);
+#pragma unroll
+        for (int l = L - 1; l >= 0; --l) {
+            const bool in = (FULL || t0 + l < q.T), on = in && (!MSK || t0 + l < ln.m.len);
+            float og[V], ox[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float G = dh[l][v] + c[v], gx = G * b[l][v];
+                ox[v] = on ? gx : 0.f;
+                og[v] = on ? gx * m[l][v] : 0.f;
+                c[v] = on ? (cut[l] ? 0.f : a[l][v] * G) : c[v];
+            }
+            if (have && in) {
+                put<T, V>(ln.dg, step_off(Step{t0, l}, op.dgate.st), ln.odg, og);
+                put<T, V>(ln.dx, step_off(Step{t0, l}, op.dx.st), ln.odx, ox);
+            }
+        }
+    };
+    int t0 = (q.T - 1) / L * L;
+    load(std::true_type{}, t0);
+    if (t0 > 0) { work(std::false_type{}, std::true_type{}, t0); t0 -= L; }
+    for (; t0 > 0; t0 -= L) work(std::true_type{}, std::true_type{}, t0);
+    work(std::false_type{}, std::false_type{}, 0);
+    if (have) op.finish(c, w.ch);
 }
 
 // One workgroup: (mean, 1 / (standard deviation + 1e-8)) of the advantages from the partials of k_scan.

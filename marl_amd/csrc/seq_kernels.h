@@ -20,6 +20,7 @@ struct ScanArgs {
     const int *lengths;
     SeqOut out, dgate, dx;          // out: h of the forward pass
     float *h_last, *dh0;
+    float *kept;                    // the states in front of every eighth step (nullable): written forward, read backward
     void *ws;
 };
 
@@ -58,6 +59,7 @@ struct ActArgs {
 };
 
 int64_t scan_workspace(int dtype, int64_t T, int64_t B, int64_t D);
+int64_t scan_kept(int dtype, int64_t T, int64_t B, int64_t D);
 int launch_scan_forward(const ScanArgs &a, hipStream_t st);
 int launch_scan_backward(const ScanArgs &a, hipStream_t st);
 int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb, float *state,

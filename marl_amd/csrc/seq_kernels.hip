@@ -110,6 +110,12 @@ int64_t scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
     return n > 1 ? (int64_t)n * 2 * B * D * 4 : 0;
 }
 
+// Bytes of the states a forward pass keeps for its backward pass, 0 where the pass reads h instead.
+int64_t scan_kept(int dtype, int64_t T, int64_t B, int64_t D)
+{
+    return D % 4 == 0 && scan_plan(T, B * D, dtype ? 2 : 4, true, true).NW == 1 ? (T + 7) / 8 * B * D * 4 : 0;
+}
+
 static ScanGeom scan_geom(const ScanArgs &a, const Plan &p)
 {
     return {(int)a.T, p.nsplit, p.Ts, (uint32_t)(a.B * a.D), (uint32_t)a.D, reinterpret_cast<float *>(a.ws)};
@@ -126,9 +132,24 @@ int launch_scan_forward(const ScanArgs &a, hipStream_t st)
     };
     const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
     return scan_dispatch<ForwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
-        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last;
+        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last; op.ck = a.kept;
         op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
     }, st);
+}
+
+template <class Op> static void fill_backward(Op &op, const ScanArgs &a)
+{
+    op.gate = a.gate; op.x = a.x; op.h = a.h; op.dh = a.dh; op.dgate = a.dgate; op.dx = a.dx;
+    op.h0 = a.h0; op.dh_last = a.dh_last; op.dh0 = a.dh0;
+    op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
+}
+template <typename T, bool MSK> static int back_kept(const ScanArgs &a, const ScanGeom &q, hipStream_t st)
+{
+    BackwardOp<T, 4, MSK, uint32_t> op;
+    fill_backward(op, a);
+    hipLaunchKernelGGL((k_scan_back_kept<T, 4, MSK>), dim3((q.C + 255) / 256), dim3(64), 0, st, op, q, a.kept);
+    LAUNCH_CHECK();
+    return 0;
 }
 
 int launch_scan_backward(const ScanArgs &a, hipStream_t st)
@@ -142,11 +163,12 @@ int launch_scan_backward(const ScanArgs &a, hipStream_t st)
                aligned(a.h0, 4 * V) && aligned(a.dh_last, 4 * V) && aligned(a.dh0, 4 * V);
     };
     const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
-    return scan_dispatch<BackwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
-        op.gate = a.gate; op.x = a.x; op.h = a.h; op.dh = a.dh; op.dgate = a.dgate; op.dx = a.dx;
-        op.h0 = a.h0; op.dh_last = a.dh_last; op.dh0 = a.dh0;
-        op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
-    }, st);
+    if (p.NW == 1 && a.kept && a.T > 0) {
+        const bool msk = a.resets || a.lengths;
+        if (a.dtype == 0) return msk ? back_kept<float, true>(a, scan_geom(a, p), st) : back_kept<float, false>(a, scan_geom(a, p), st);
+        return msk ? back_kept<bf16, true>(a, scan_geom(a, p), st) : back_kept<bf16, false>(a, scan_geom(a, p), st);
+    }
+    return scan_dispatch<BackwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) { fill_backward(op, a); }, st);
 }
 
 int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb, float *state,

@@ -96,30 +96,31 @@ def _explain_scan(gate, x, h0, resets, lengths, B, D):
     _on_device(fn, gate.device, x, h0, resets, lengths)
 
 
-def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D):
-    dev, dt = gate.device, _DTYPES[gate.dtype]
+def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D, keep=False):
+    dev, dt, lib = gate.device, _DTYPES[gate.dtype], _lib.load()
     h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
     last = torch.empty((B, D), dtype=torch.float32, device=dev)
-    need = _lib.load().asm_gated_scan_workspace(dt, T, B, D)
+    need = lib.asm_gated_scan_workspace(dt, T, B, D)
     ws = _workspace(need, dev)
+    kept = _workspace(lib.asm_gated_scan_kept(dt, T, B, D), dev) if keep else None
     _call("asm_gated_scan_forward", dev, dt, T, B, D, *_tb(gate, batch_first), *_tb(x, batch_first), _ptr(h0), *_tb(resets, batch_first),
-          _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(ws), need)
-    return h, last
+          _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(kept), _ptr(ws), need)
+    return h, last, kept
 
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, gate, x, h0, resets, lengths, batch_first, dims):
         ctx.set_materialize_grads(False)
-        h, last = _scan_forward(gate, x, h0, resets, lengths, batch_first, *dims)
-        ctx.save_for_backward(gate, x, h, h0, resets, lengths)
+        h, last, kept = _scan_forward(gate, x, h0, resets, lengths, batch_first, *dims, keep=True)
+        ctx.save_for_backward(gate, x, h, h0, resets, lengths, kept)
         ctx.batch_first, ctx.dims = batch_first, dims
         return h, last
 
     @staticmethod
     def backward(ctx, dh, dlast):
         _once("gated_scan")
-        gate, x, h, h0, resets, lengths = ctx.saved_tensors
+        gate, x, h, h0, resets, lengths, kept = ctx.saved_tensors
         T, B, D = ctx.dims
         bf, dev, dt = ctx.batch_first, gate.device, _DTYPES[gate.dtype]
         dh = None if dh is None else _dense(dh)
@@ -130,7 +131,7 @@ class _GatedScan(torch.autograd.Function):
         need = _lib.load().asm_gated_scan_workspace(dt, T, B, D)
         ws = _workspace(need, dev)
         _call("asm_gated_scan_backward", dev, dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf), _ptr(lengths),
-              *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0), _ptr(ws), need)
+              *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0), _ptr(kept), _ptr(ws), need)
         return dgate, dx, dh0, None, None, None, None
 
 
@@ -157,7 +158,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
         h, last = _GatedScan.apply(gate, x, h0, resets, lengths, batch_first, (T, B, D))
         return _guard_leaves(h, h.device), last
-    return _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D)
+    return _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D)[:2]
 
 
 def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, reset: Optional[torch.Tensor] = None,

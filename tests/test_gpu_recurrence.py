@@ -20,7 +20,8 @@ def no_garbage():
 
 
 SHAPES = [(1, 1, 1), (0, 3, 5), (3, 2, 64), (31, 3, 7), (32, 1, 65), (33, 2, 12), (100, 5, 61), (200, 64, 30),
-          (9, 300, 256), (67, 280, 256), (40, 1100, 61), (1000, 2, 5), (4099, 1, 3), (700, 3, 256)]
+          (9, 300, 256), (67, 280, 256), (40, 1100, 61), (1000, 2, 5), (4099, 1, 3), (700, 3, 256),
+          (1, 1200, 256), (8, 1200, 256), (21, 601, 256), (24, 1200, 256), (35, 1201, 256), (600, 1, 64), (90, 20, 64)]
 
 
 def _make(torch, T, B, D, dtype, batch_first, seed, resets=False, lengths=False, h0=False):

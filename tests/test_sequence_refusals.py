@@ -115,16 +115,17 @@ def test_c_abi_refuses_before_it_launches():
     """Made-up addresses: a call that got as far as a launch would fail differently."""
     lib = _lib.load()
     p = 1 << 20
-    fwd = lambda dt=0, T=T, B=B, D=D, gate=p, x=p, h=p, ws=None, n=0: lib.asm_gated_scan_forward(  # noqa: E731
-        dt, T, B, D, gate, 0, 0, x, 0, 0, None, None, 0, 0, None, h, 0, 0, None, ws, n, None)
+    fwd = lambda dt=0, T=T, B=B, D=D, gate=p, x=p, h=p, ws=None, n=0, kept=None: lib.asm_gated_scan_forward(  # noqa: E731
+        dt, T, B, D, gate, 0, 0, x, 0, 0, None, None, 0, 0, None, h, 0, 0, None, kept, ws, n, None)
     for kw, msg in ((dict(dt=7), "dtype"), (dict(T=-1), "negative"), (dict(B=1 << 31), "too large"), (dict(B=1 << 29, D=2), "too large"), (dict(B=1 << 20, D=1 << 20), "too large"),
                     (dict(T=1 << 31), "too large"), (dict(gate=None), "NULL"), (dict(x=None), "NULL"), (dict(h=None), "NULL"),
-                    (dict(T=100000), "workspace"), (dict(T=100000, ws=p, n=8), "workspace"), (dict(T=100000, ws=p + 8, n=1 << 40), "aligned")):
+                    (dict(T=100000), "workspace"), (dict(T=100000, ws=p, n=8), "workspace"), (dict(T=100000, ws=p + 8, n=1 << 40), "aligned"), (dict(kept=p + 4), "kept")):
         assert fwd(**kw) != 0 and msg in _msg(lib), (kw, _msg(lib))
     assert fwd(B=0, gate=None, x=None, h=None) == 0                     # nothing to do
     assert lib.asm_gated_scan_workspace(0, 100000, B, D) > 0 and lib.asm_gated_scan_workspace(0, -1, B, D) < 0
+    assert lib.asm_gated_scan_kept(0, 20, B, D) == 0 and lib.asm_gated_scan_kept(0, 20, 600, 256) == 3 * 600 * 256 * 4 and lib.asm_gated_scan_kept(5, 20, B, D) < 0
     bwd = lambda T=T, dgate=p, h=p: lib.asm_gated_scan_backward(0, T, B, D, p, 0, 0, p, 0, 0, h, 0, 0, None, None, 0, 0, None, None, 0, 0, None,  # noqa: E731
-                                                                dgate, 0, 0, p, 0, 0, None, None, 0, None)
+                                                                dgate, 0, 0, p, 0, 0, None, None, None, 0, None)
     assert bwd(dgate=None) != 0 and "NULL" in _msg(lib)
     assert bwd(h=None) != 0 and "NULL" in _msg(lib)
     assert bwd(T=100000) != 0 and "workspace" in _msg(lib)
