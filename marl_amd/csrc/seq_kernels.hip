@@ -33,12 +33,13 @@ struct Plan { int V, NW, L, nsplit, Ts; };
 // By C, the channels, and `size`, the bytes of a value (forward + backward of 200 steps, float32 / bfloat16, us):
 //   C       1 channel a lane, 4 waves a tile   2 channels, 4 waves   4 channels, one wave walks all of time
 //   30720              39 / 32                      41 / 32                     110 / 114
-//   62848              77 / 49                      75 / 42                     128 / 114
-//   122880            179 / 97                     164 / 80                     172 / 145
-//   245760            361 / 205                    359 / 176                    312 / 182
-//   491520            706 / 401                    695 / 359                    676 / 325
-// Many channels fill the chip by themselves, and a wave that shares nothing waits for nobody: from 600 KB a time step on.  Below,
-// four waves side by side in time; from 49152 channels on two of them in a lane (half the address work).  Rows that are not aligned to two or four
+//   62848              77 / 49                      75 / 42                     105 / 96
+//   122880            179 / 97                     162 / 79                     157 / 109
+//   245760            361 / 205                    357 / 174                    292 / 161
+//   491520            706 / 401                    691 / 358                    613 / 315
+// Many channels fill the chip by themselves, a wave that shares nothing waits for nobody, and its backward pass needs not read
+// h (k_scan_back_kept): from 480 KB a time step on.  Below, four waves side by side in time; from 49152 channels on two of
+// them in a lane (half the address work).  Rows that are not aligned to two or four
 // values go one channel a lane.
 // Fewer than 256 workgroups of one channel a lane: what counts is how often a tile's loads are waited for.  Up to `whole` steps eight
 // waves share a tile and one launch does it all; from there on the time axis is cut until there are 512 workgroups, down to one tile
@@ -48,7 +49,7 @@ struct Plan { int V, NW, L, nsplit, Ts; };
 Plan scan_plan(int64_t T, int64_t C, size_t size, bool vec2, bool vec4, int64_t whole = 320)
 {
     Plan p{1, 4, 8, 1, 0};
-    if (vec4 && C * (int64_t)size >= 600000) p = {4, 1, 4, 1, 0};
+    if (vec4 && C * (int64_t)size >= 480000) p = {4, 1, 4, 1, 0};
     else if (vec2 && C >= 49152) p = {2, 4, 4, 1, 0};
     const int64_t groups = (C + 64 * p.V - 1) / (64 * p.V);
     const bool few = p.V == 1 && groups < 256;

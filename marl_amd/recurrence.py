@@ -9,6 +9,7 @@ of DeviceReplay hold; batch_first=True takes (B, T, D).  Tensors may be strided 
 (others are copied).  No CPU fallback."""
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -96,13 +97,20 @@ def _explain_scan(gate, x, h0, resets, lengths, B, D):
     _on_device(fn, gate.device, x, h0, resets, lengths)
 
 
+@lru_cache(maxsize=1024)
+def _scan_sizes(dt: int, T: int, B: int, D: int) -> Tuple[int, int]:
+    """(workspace, kept states) in bytes: functions of the sizes alone."""
+    lib = _lib.load()
+    return lib.asm_gated_scan_workspace(dt, T, B, D), lib.asm_gated_scan_kept(dt, T, B, D)
+
+
 def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D, keep=False):
-    dev, dt, lib = gate.device, _DTYPES[gate.dtype], _lib.load()
+    dev, dt = gate.device, _DTYPES[gate.dtype]
     h = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
     last = torch.empty((B, D), dtype=torch.float32, device=dev)
-    need = lib.asm_gated_scan_workspace(dt, T, B, D)
+    need, states = _scan_sizes(dt, T, B, D)
     ws = _workspace(need, dev)
-    kept = _workspace(lib.asm_gated_scan_kept(dt, T, B, D), dev) if keep else None
+    kept = _workspace(states, dev) if keep else None
     _call("asm_gated_scan_forward", dev, dt, T, B, D, *_tb(gate, batch_first), *_tb(x, batch_first), _ptr(h0), *_tb(resets, batch_first),
           _ptr(lengths), *_tb(h, batch_first), last.data_ptr(), _ptr(kept), _ptr(ws), need)
     return h, last, kept
@@ -128,7 +136,7 @@ class _GatedScan(torch.autograd.Function):
         dgate = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         dx = torch.empty(gate.shape, dtype=gate.dtype, device=dev)
         dh0 = torch.empty((B, D), dtype=torch.float32, device=dev) if ctx.needs_input_grad[2] else None
-        need = _lib.load().asm_gated_scan_workspace(dt, T, B, D)
+        need = _scan_sizes(dt, T, B, D)[0]
         ws = _workspace(need, dev)
         _call("asm_gated_scan_backward", dev, dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf), _ptr(lengths),
               *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0), _ptr(kept), _ptr(ws), need)
