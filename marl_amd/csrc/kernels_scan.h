@@ -38,6 +38,20 @@ template <typename T, int V> __device__ __forceinline__ void store_vec(void *p, 
     *reinterpret_cast<Pack<T, V> *>(reinterpret_cast<T *>(p) + off) = r;
 }
 
+// The [B][D] arrays in front of and behind a sequence, of any alignment (read and written once).
+template <int V> __device__ __forceinline__ void load_each(float (&o)[V], const float *p, uint32_t ch)
+{
+#pragma unroll
+    for (int v = 0; v < V; ++v) o[v] = p ? p[ch + v] : 0.f;
+}
+template <int V> __device__ __forceinline__ void store_each(float *p, uint32_t ch, const float (&x)[V])
+{
+    if (p) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[ch + v] = x[v];
+    }
+}
+
 // a = sigmoid(g) and b = 1 - a from e = exp(-g): a = 1 / (1 + e), b = e a where e < 1 and 1 - a elsewhere, so neither end
 // loses digits and nothing is infinite times zero.  The exponential and the reciprocal are the hardware's (1 unit in the
 // last place each); what remains is the rounding of g log2(e), |g| units of e: with the sums, a and b are good to 4 + |g|
@@ -139,12 +153,7 @@ template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
         if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
-    __device__ void carry0(float (&c)[V], int64_t ch) const
-    {
-#pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = 0.f;
-        if (h0) load_vec<float, V>(c, h0, ch);
-    }
+    __device__ void carry0(float (&c)[V], uint32_t ch) const { load_each(c, h0, ch); }
     __device__ void load(Raw &i, const Lane &l, const Step &s, bool) const
     {
         fetch(i.g, l.g, step_off(s, gate.st), l.og);
@@ -175,7 +184,7 @@ template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
         }
         if (on) put<T, V>(l.o, step_off(s, out.st), l.oo, o);
     }
-    __device__ void finish(const float (&c)[V], int64_t ch) const { if (h_last) store_vec<float, V>(h_last, ch, c); }
+    __device__ void finish(const float (&c)[V], uint32_t ch) const { store_each(h_last, ch, c); }
 };
 
 template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
@@ -196,12 +205,7 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
         if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
-    __device__ void carry0(float (&c)[V], int64_t ch) const
-    {
-#pragma unroll
-        for (int v = 0; v < V; ++v) c[v] = 0.f;
-        if (dh_last) load_vec<float, V>(c, dh_last, ch);
-    }
+    __device__ void carry0(float (&c)[V], uint32_t ch) const { load_each(c, dh_last, ch); }
     // agg: only what the composition needs
     __device__ void load(Raw &i, const Lane &l, const Step &s, bool agg) const
     {
@@ -218,11 +222,7 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
         float before[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) before[v] = i.h.get(v);
-        if (s.t() == 0) {                                                    // (uniform)
-#pragma unroll
-            for (int v = 0; v < V; ++v) before[v] = 0.f;
-            if (h0) load_vec<float, V>(before, h0, l.ch);
-        }
+        if (s.t() == 0) load_each(before, h0, l.ch);                     // (uniform)
         if (MSK) on = on && s.t() < l.m.len;
         o.cut = MSK && on && i.cut.get(0);
 #pragma unroll
@@ -254,7 +254,7 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
             put<T, V>(l.dx, step_off(s, dx.st), l.odx, ox);
         }
     }
-    __device__ void finish(const float (&c)[V], int64_t ch) const { if (dh0) store_vec<float, V>(dh0, ch, c); }
+    __device__ void finish(const float (&c)[V], uint32_t ch) const { store_each(dh0, ch, c); }
 };
 
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.

@@ -93,6 +93,8 @@ def test_loss_of_replay_views(torch_cuda):
     _check(torch, mean, std, act, old, one, old, None, what="expanded")
     m2 = torch.randn(T, E, n, 3 * A, device="cuda")[..., 1::3]
     _check(torch, m2, std, act, old, adv, None, None, what="strided mean")
+    _check(torch, mean, std, act, old, adv, ref, mask, clip=1.5, what="clip beyond 1")
+    _check(torch, mean[0, 0, 0], std, act[0, 0, 0], old[0, 0, 0], adv[0, 0, 0], ref[0, 0, 0], None, what="one row, no axes")
     both = torch.randn(T, E, n, 2 * A, device="cuda") * 0.3             # one head's output, cut in two
     _check(torch, both[..., :A], both[..., A:], act, old, adv, ref, mask, what="cut head")
 

@@ -65,13 +65,19 @@ def test_scan_matches_the_64_bit_form(torch_cuda, T, B, D, dtype, marks):
 def test_scan_takes_strided_tensors(torch_cuda, dtype):
     torch = torch_cuda
     dt = getattr(torch, dtype)
-    for T, B, D in ((50, 6, 24), (20, 300, 256)):
+    for T, B, D in ((50, 6, 24), (20, 300, 256), (11, 1200, 256)):
         both = torch.randn(T, B, 2 * D + 3, device="cuda").to(dt)      # one projection's output, cut in two
         _check(torch, both[..., :D], both[..., D + 3:], None, None, None, False, what="cut projection")
         _check(torch, both[..., 1:D + 1], both[..., D:2 * D], None, None, None, False, what="odd offset")
         _check(torch, both[..., :D].transpose(0, 1), both[..., :D].transpose(0, 1), None, None, None, True, what="transposed")
         one = torch.randn(T, 1, D, device="cuda").to(dt)                # a gate shared by all sequences
         _check(torch, one.expand(T, B, D), both[..., :D], None, torch.rand(1, B, device="cuda").expand(T, B) < 0.3, None, False, what="expanded")
+        four = torch.randn(T, B, 2 * D + 4, device="cuda").to(dt)       # aligned rows, further apart than their length
+        far0 = torch.randn(B * D + 1, device="cuda")[1:].view(B, D)     # a state that is aligned to nothing
+        n = torch.randint(-3, T + 4, (B,), device="cuda", dtype=torch.int32)       # (lengths are clamped)
+        _check(torch, four[..., :D], four[..., D:2 * D], far0, torch.rand(T, B, device="cuda") < 0.1, n, False, what="aligned cut")
+        flat = torch.randn(1, 1, D, device="cuda").to(dt)               # one decay for all steps
+        _check(torch, flat.expand(T, B, D), four[..., :D], far0, None, None, False, what="one gate")
         wide = torch.randn(T, B, 2 * D, device="cuda").to(dt)[..., ::2]  # last axis not contiguous: copied
         _check(torch, wide, wide, None, None, None, False, what="step of two")
 
