@@ -10,7 +10,9 @@
 // What is in double and what is not: z, log_pi, d and q = e^d are in double, and so is the decision whether a ratio lies beyond the
 // clipping border (d against log(1 +- eps): it decides between a gradient and none) and the sum of the gains, whose terms
 // cancel.  e^D - 1 - D, which cancels for nearly equal policies, is its own series where |D| < 1, in float32; so are the
-// products behind the row's gradient.  Sums are in double.
+// products behind the row's gradient.  Sums are in double.  Measured at 24.6 M rows of two components: 167 us for 787 MB, 4.7 TB/s (a copy of
+// 2 GiB reaches 4.95), 180 vector instructions a row, 0.55 of the issue; every row wholly in double: 189 us, bound by its instructions.
+// 2048 rows in one workgroup: 9 us, its two trips to memory and one long chain of dependent double operations a row.
 // The gradients are written in the same pass as the loss: a mean over rows needs only their count, known without a mask
 // and counted ahead with one.  Sums: per thread, per workgroup in a fixed order, then over the workgroups in a fixed order:
 // the same inputs give the same bits.
@@ -347,6 +349,7 @@ template <typename TM> __global__ __launch_bounds__(256) void k_policy_loss_scal
 
 struct ActDev { uint32_t rows, n; int A; Rows mean, log_std, noise, actions, log_pi; };
 
+// 4096 x 30 rows: 3.7 us, 30 rows: 2.0 us (a launch).
 // u = mu + e^s noise (or the given u), and the log-probability of u as it is stored.
 template <typename TM, bool DRAW> __global__ __launch_bounds__(256) void k_gaussian_act(ActDev p)
 {
