@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import math
 import struct
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -95,36 +96,41 @@ def _explain_policy(fn, mean, log_std, full, per_row):
 
 class _ClippedLoss(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl_coef, entropy_coef):
+    def forward(ctx, mean, log_std, fixed, options):                    # fixed: the tensors without a gradient
         ctx.set_materialize_grads(False)
-        loss, stats, dmean, dstd = _loss(mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl_coef, entropy_coef)
-        ctx.grads, ctx.args = (dmean, dstd), (shared, clip, kl_coef, entropy_coef)
-        ctx.save_for_backward(mean, log_std, actions, old, ref, adv, mask, moments)
+        loss, stats, dmean, dstd = _loss(mean, log_std, *fixed, *options)
+        ctx.grads, ctx.options = (dmean, dstd), options
+        ctx.save_for_backward(mean, log_std, *fixed)
         ctx.mark_non_differentiable(stats)
         return loss, stats
 
     @staticmethod
     def backward(ctx, g, _):
-        none = (None,) * 10
         if g is None:
-            return (None, None) + none
+            return None, None, None, None
         _once("clipped_policy_loss")
         # the gradients of the forward pass are handed out once; a second backward pass over a retained graph makes its own
         tensors = ctx.saved_tensors                                     # (notices inputs overwritten since)
         grads, ctx.grads = ctx.grads, None
-        dmean, dstd = grads if grads is not None else _loss(*tensors, *ctx.args)[2:]
+        dmean, dstd = grads if grads is not None else _loss(*tensors, *ctx.options)[2:]
         _call("asm_policy_loss_scale", dmean.device, _DTYPES[dmean.dtype], g.data_ptr(), dmean.numel(), dmean.data_ptr(), dstd.numel(), dstd.data_ptr())
-        return (dmean, dstd) + none
+        return dmean, dstd, None, None
+
+
+@lru_cache(maxsize=1024)
+def _loss_workspace(rows: int, A: int) -> int:
+    return _lib.load().asm_policy_loss_workspace(rows, A)
 
 
 def _loss(mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl_coef, entropy_coef):
     dev, shape, dt = mean.device, mean.shape, mean.dtype
     lead, A = len(shape) - 1, shape[-1]
     B, n = _dims(shape[:-1])
-    out = torch.empty(7, dtype=torch.float32, device=dev)
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    stats = torch.empty(6, dtype=torch.float32, device=dev)
     dmean = torch.empty(shape, dtype=dt, device=dev)
     dstd = torch.empty(log_std.shape, dtype=dt, device=dev)
-    need = _lib.load().asm_policy_loss_workspace(B * n, A)
+    need = _loss_workspace(B * n, A)
     ws = _workspace(need, dev)
     r0, k0 = _rows(mean, lead, True)                                    # (k: the tensors a copy may have been made of)
     r1, k1 = _rows_std(log_std, lead, shared)
@@ -133,10 +139,9 @@ def _loss(mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl
     r4, k4 = _rows(ref, lead, False) if ref is not None else (_NO_ROWS, None)
     r5, k5 = _rows(adv, lead, False)
     r6, k6 = _rows(mask, lead, False) if mask is not None else (_NO_ROWS, None)
-    at = out.data_ptr()
     _call("asm_policy_loss", dev, _DTYPES[dt], B, n, A, shared, _pack_loss(*r0, *r1, *r2, *r3, *r4, *r5, *r6), _ptr(moments), clip, kl_coef,
-          entropy_coef, at, at + 4, dmean.data_ptr(), dstd.data_ptr(), _ptr(ws), need)
-    return out[0], out[1:], dmean, dstd
+          entropy_coef, loss.data_ptr(), stats.data_ptr(), dmean.data_ptr(), dstd.data_ptr(), _ptr(ws), need)
+    return loss, stats, dmean, dstd
 
 
 def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Tensor, log_pi_old: torch.Tensor, adv: torch.Tensor, *,
@@ -164,7 +169,8 @@ def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torc
         _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv_moments, clip, kl_coef, entropy_coef)
     shared = int(log_std.shape == mean.shape[-1:])
     adv_moments = None if adv_moments is None else adv_moments.contiguous()
-    loss, stats = _ClippedLoss.apply(mean, log_std, actions, log_pi_old, log_pi_ref, adv, mask, adv_moments, shared, float(clip), float(kl_coef), float(entropy_coef))
+    loss, stats = _ClippedLoss.apply(mean, log_std, (actions, log_pi_old, log_pi_ref, adv, mask, adv_moments),
+                                     (shared, float(clip), float(kl_coef), float(entropy_coef)))
     return (_guard_leaves(loss, mean.device) if loss.requires_grad else loss), stats
 
 

@@ -118,10 +118,10 @@ def _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D, keep=False
 
 class _GatedScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, gate, x, h0, resets, lengths, batch_first, dims):
+    def forward(ctx, gate, x, h0, marks, batch_first, dims):
         ctx.set_materialize_grads(False)
-        h, last, kept = _scan_forward(gate, x, h0, resets, lengths, batch_first, *dims, keep=True)
-        ctx.save_for_backward(gate, x, h, h0, resets, lengths, kept)
+        h, last, kept = _scan_forward(gate, x, h0, *marks, batch_first, *dims, keep=True)
+        ctx.save_for_backward(gate, x, h, h0, *marks, kept)
         ctx.batch_first, ctx.dims = batch_first, dims
         return h, last
 
@@ -140,7 +140,7 @@ class _GatedScan(torch.autograd.Function):
         ws = _workspace(need, dev)
         _call("asm_gated_scan_backward", dev, dt, T, B, D, *_tb(gate, bf), *_tb(x, bf), *_tb(h, bf), _ptr(h0), *_tb(resets, bf), _ptr(lengths),
               *_tb(dh, bf), _ptr(dlast), *_tb(dgate, bf), *_tb(dx, bf), _ptr(dh0), _ptr(kept), _ptr(ws), need)
-        return dgate, dx, dh0, None, None, None, None
+        return dgate, dx, dh0, None, None, None
 
 
 def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] = None, *, resets: Optional[torch.Tensor] = None,
@@ -164,7 +164,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     h0 = None if h0 is None else h0.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
     if torch.is_grad_enabled() and (gate.requires_grad or x.requires_grad or (h0 is not None and h0.requires_grad)):
-        h, last = _GatedScan.apply(gate, x, h0, resets, lengths, batch_first, (T, B, D))
+        h, last = _GatedScan.apply(gate, x, h0, (resets, lengths), batch_first, (T, B, D))
         return _guard_leaves(h, h.device), last
     return _scan_forward(gate, x, h0, resets, lengths, batch_first, T, B, D)[:2]
 
