@@ -366,7 +366,8 @@ int asm_policy_mlp_act_bf16(int E, int n_a, int obs_dim, int hidden, int act_dim
  * size the matching *_workspace function returns (aligned to 16 bytes; NULL where that is 0), free again once the stream
  * has passed the call; two calls that may run at the same time need two.
  * dtype: ASM_SEQ_F32 or ASM_SEQ_BF16, the type of gate, x, h and their gradients, or of mean, log_std and theirs; all
- * other floating arrays are float32.  Strides are in elements.  Outputs must not overlap inputs or each other. */
+ * other floating arrays are float32.  Strides are in elements and may be 0 (inputs) or negative.  Outputs must not overlap inputs or
+ * each other. */
 #define ASM_SEQ_F32 0
 #define ASM_SEQ_BF16 1
 

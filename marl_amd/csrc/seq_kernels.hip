@@ -94,11 +94,14 @@ int scan_dispatch(int dtype, bool msk, const Plan &p, bool far, const ScanGeom &
     return msk ? scan_typed<Op, bf16, true>(p, far, q, fill, st) : scan_typed<Op, bf16, false>(p, far, q, fill, st);
 }
 
-// Whether a workgroup's sequences lie too far apart for 32-bit byte offsets (V: the most channels a lane may take).
+// Whether a workgroup's sequences lie too far apart, or backwards, for unsigned 32-bit byte offsets.
 bool too_far(int64_t D, std::initializer_list<int64_t> strides, size_t elem)
 {
     int64_t sb = 0;
-    for (int64_t s : strides) sb = std::max(sb, s);
+    for (int64_t s : strides) {
+        if (s < 0) return true;
+        sb = std::max(sb, s);
+    }
     const int64_t rows = 64 * 4 / D + 2;
     return (double)rows * (double)sb * (double)elem + (double)D * (double)elem >= 4294967296.0;
 }

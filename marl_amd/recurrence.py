@@ -182,13 +182,20 @@ def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *,
             state.is_contiguous() and not ((state.requires_grad or (out is not None and out.requires_grad)) and torch.is_grad_enabled()) and
             (reset is None or (reset.shape == shape[:1] and reset.dtype in _FLAGS and reset.device == dev)) and dev.type == "cuda" and
             x.device == dev and state.device == dev and out.device == dev and out.shape == shape and out.dtype == dt and
-            (D <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= D) and (out.data_ptr() != state.data_ptr() or shape.numel() == 0)):
+            (D <= 1 or out.stride(1) == 1) and (shape[0] <= 1 or out.stride(0) >= D) and _apart(state, out)):
         _explain_step(gate, x, state, reset, out)
     gate, x = _dense(gate), _dense(x)
     _call("asm_gated_scan_step", dev, _DTYPES[dt], shape[0], D, gate.data_ptr(), gate.stride(0), x.data_ptr(), x.stride(0), state.data_ptr(),
           _ptr(reset), 0 if reset is None else reset.stride(0), out.data_ptr(), out.stride(0))
     torch.autograd.graph.increment_version((state, out))                # (written behind autograd's back)
     return out
+
+
+def _apart(state, out) -> bool:
+    """Whether a contiguous state and the rows of out lie in different memory (with the rows' gaps)."""
+    s, o = state.data_ptr(), out.data_ptr()
+    B, D = out.shape
+    return o >= s + state.nbytes or o + ((B - 1) * out.stride(0) + D) * out.element_size() <= s or B * D == 0
 
 
 def _explain_step(gate, x, state, reset, out):
@@ -203,7 +210,7 @@ def _explain_step(gate, x, state, reset, out):
                           and not (out.requires_grad and torch.is_grad_enabled())),
           f"{fn}: out must be a tensor of gate's shape and type with contiguous rows that do not overlap")
     _on_device(fn, gate.device, x, state, reset, out)
-    raise ValueError(f"{fn}: out and state must be two tensors")
+    raise ValueError(f"{fn}: out and state must not share memory")
 
 
 def _time_rows(t: torch.Tensor) -> torch.Tensor:

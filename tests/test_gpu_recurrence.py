@@ -351,3 +351,47 @@ def test_second_derivatives_are_refused(torch_cuda):
     mean, row = torch.randn(6, 2, device="cuda", requires_grad=True), torch.randn(6, device="cuda")
     with pytest.raises(RuntimeError, match="differentiable once"):
         torch.autograd.grad(clipped_policy_loss(mean, torch.zeros(2, device="cuda"), mean.detach(), row, row)[0], mean, create_graph=True)
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_c_entries_take_sequences_in_reverse_order(torch_cuda, D):
+    """Strides of the C entries may be negative: the batch, or time, read from its far end."""
+    torch = torch_cuda
+    from marl_amd import _lib
+    lib, T, B = _lib.load(), 19, 500
+    gate, x, dh = (torch.randn(T, B, D, device="cuda") for _ in range(3))
+    cut = (torch.rand(T, B, device="cuda") < 0.1).to(torch.uint8)
+    for axis in (0, 1):
+        h, dgate, dx = (torch.zeros_like(gate) for _ in range(3))
+
+        def at(t):
+            s = list(t.stride()[:2])
+            first = t.data_ptr() + (t.shape[axis] - 1) * s[axis] * t.element_size()
+            s[axis] = -s[axis]
+            return (first, *s)
+        st = torch.cuda.current_stream().cuda_stream
+        need = lib.asm_gated_scan_workspace(0, T, B, D)
+        ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+        kept = lib.asm_gated_scan_kept(0, T, B, D)
+        kept = torch.empty(kept, dtype=torch.uint8, device="cuda") if kept else None
+        pk = None if kept is None else kept.data_ptr()
+        _lib.check(lib.asm_gated_scan_forward(0, T, B, D, *at(gate), *at(x), None, *at(cut), None, *at(h), None, pk, ws.data_ptr(), need, st), "forward")
+        _lib.check(lib.asm_gated_scan_backward(0, T, B, D, *at(gate), *at(x), *at(h), None, *at(cut), None, *at(dh), None, *at(dgate), *at(dx), None, pk,
+                                               ws.data_ptr(), need, st), "backward")
+        turned = lambda t: t.flip(axis)  # noqa: E731
+        want = so.scan(turned(gate), turned(x), resets=turned(cut) != 0, dh=turned(dh))
+        for name, got in (("h", h), ("dgate", dgate), ("dx", dx)):
+            so.within(turned(got), *want[name], f"axis {axis} {name}")
+
+
+def test_step_refuses_outputs_on_its_state(torch_cuda):
+    torch = torch_cuda
+    from marl_amd.recurrence import gated_scan_step
+    gate, x, buf = torch.randn(6, 8, device="cuda"), torch.randn(6, 8, device="cuda"), torch.zeros(20, 8, device="cuda")
+    for out in (buf[4:10], buf[9:15], buf.view(10, 16)[2:8, :8]):       # state: rows 4 to 9
+        with pytest.raises(ValueError, match="share memory"):
+            gated_scan_step(gate, x, buf[4:10], out=out)
+    assert not buf.any()
+    want = gated_scan_step(gate, x, torch.zeros(6, 8, device="cuda"))
+    gated_scan_step(gate, x, buf[4:10], out=buf[10:16])                 # one buffer, different rows
+    assert torch.equal(buf[10:16], want) and torch.equal(buf[4:10], want) and not buf[:4].any() and not buf[16:].any()
