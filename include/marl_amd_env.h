@@ -377,8 +377,10 @@ int asm_policy_mlp_act_bf16(int E, int n_a, int obs_dim, int hidden, int act_dim
  * where nonzero, the state in front of step t counts as zero, whatever it holds.  lengths (nullable, [B], clamped to
  * 0..T): steps from lengths[b] on are not part of the sequence: h is zero there, the state passes.  h_last
  * (nullable): [B][D], the state behind the last step.  h0, h_last, dh0, dh_last: [B][D] contiguous.
- * kept (nullable): asm_gated_scan_kept bytes (aligned to 16) in which the forward pass leaves the states in front of every eighth
- * step for the backward pass of the same arguments, which then reads those and not h: where that function returns 0, pass NULL. */
+ * kept (nullable): asm_gated_scan_kept bytes (aligned to 16) in which the forward pass leaves the float32 states in front of every
+ * eighth step, counted from the last, for the backward pass of the same arguments, which then works from those and not from h: where
+ * that function returns 0, pass NULL.  A bfloat16 backward pass without them takes the states from h as it is stored: the gate's
+ * gradient, a product with h_{t-1} - x_t, is then off by half a step of h in place of that difference's own. */
 int64_t asm_gated_scan_kept(int dtype, int64_t T, int64_t B, int64_t D);
 int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D);
 int asm_gated_scan_forward(int dtype, int64_t T, int64_t B, int64_t D, const void *gate, int64_t gate_st, int64_t gate_sb,

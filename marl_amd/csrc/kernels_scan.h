@@ -140,12 +140,12 @@ template <typename T, int V, typename OFF> __device__ __forceinline__ void put(c
 // is written).
 
 template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
-    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = true;
+    static constexpr bool REVERSE = false, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = true, BLOCK = false;
     Seq gate, x;
     SeqOut out;
     const float *h0;
     float *h_last;
-    float *ck;                                                          // the state in front of every eighth step, [T / 8][C] (nullable)
+    float *ck;                                                          // (nullable) the state in front of step T - 8 (k + 1), at [k][channel]
     Marks marks;
     struct Lane { const char *g, *x, *o, *r; OFF og, ox, oo; MarkLane<OFF> m; };
     struct Raw { Words<T, V> g, x; Words<uint8_t, 1> cut; };
@@ -157,6 +157,7 @@ template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
         if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
+    ForwardOp composing() const { return *this; }                       // (the operator of a launch that only composes)
     __device__ void carry0(float (&c)[V], uint32_t ch) const { load_each(c, h0, ch); }
     __device__ void load(Raw &i, const Lane &l, const Step &s, bool) const
     {
@@ -191,12 +192,17 @@ template <typename T, int V, bool MSK, typename OFF> struct ForwardOp {
     __device__ void finish(const float (&c)[V], uint32_t ch) const { store_each(h_last, ch, c); }
 };
 
-template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
-    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = false;
+// KEPT: the states in front of a wave's eight steps come from what the forward pass kept and are computed again in between, in
+// float32, from the gates and inputs the pass reads anyway; else they are h as it is stored.  h in bfloat16 would give the
+// gate's gradient, a product with h_{t-1} - x_t, an error of half a step of h: as much as the difference itself where the
+// memory has settled near its input.
+template <typename T, int V, bool MSK, typename OFF, bool KEPT> struct BackwardAnyOp {
+    static constexpr bool REVERSE = true, SUMS = false, MOMENTS = false, CUTS = MSK, KEEPS = false, BLOCK = KEPT;
     Seq gate, x, h, dh;
     SeqOut dgate, dx;
     const float *h0, *dh_last;
     float *dh0;
+    const float *ck;
     Marks marks;
     struct Lane { const char *g, *x, *h, *dh, *dg, *dx, *r; OFF og, ox, oh, odh, odg, odx; uint32_t ch; MarkLane<OFF> m; };
     struct Raw { Words<T, V> g, x, h, dh; Words<uint8_t, 1> cut; };
@@ -209,6 +215,7 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
         if (MSK) l.m = mark_lane<OFF>(marks, w, q.T);
         return l;
     }
+    BackwardAnyOp<T, V, MSK, OFF, false> composing() const { return {gate, x, h, dh, dgate, dx, h0, dh_last, dh0, ck, marks}; }      // (needs no states)
     __device__ void carry0(float (&c)[V], uint32_t ch) const { load_each(c, dh_last, ch); }
     // agg: only what the composition needs
     __device__ void load(Raw &i, const Lane &l, const Step &s, bool agg) const
@@ -218,11 +225,51 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
         if (MSK) { i.cut.w = 0; if (marks.resets) fetch(i.cut, l.r, step_off(s, marks.r_st), l.m.r); }
         if (!agg) {
             fetch(i.x, l.x, step_off(s, x.st), l.ox);
-            fetch(i.h, l.h, s.t() > 0 ? step_off(Step{s.tb, s.dl - 1}, h.st) : 0, l.oh);
+            if (!KEPT) fetch(i.h, l.h, s.t() > 0 ? step_off(Step{s.tb, s.dl - 1}, h.st) : 0, l.oh);
+        }
+    }
+    // The state in front of the eight steps u0 .. u0 + 7 from the end (uniform).
+    __device__ void load_state(float (&o)[V], const ScanGeom &q, int u0, uint32_t ch) const
+    {
+        if (u0 + 8 <= q.T) load_vec<float, V>(o, ck, (int64_t)(u0 / 8) * q.C + ch);
+        else load_each(o, h0, ch);                                      // (the block that reaches the first step)
+    }
+    // Forwards through the block, whose step k lies k in front of `last`; steps from `n` on lie in front of the first one.
+    template <int L> __device__ void states(Item (&o)[L], const Raw (&raw)[L], const float (&state)[V], const Lane &l, int last, int n) const
+    {
+        float before[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) before[v] = state[v];
+#pragma unroll
+        for (int k = L - 1; k >= 0; --k) {
+            const bool on = k < n && (!MSK || last - k < l.m.len), cut = MSK && raw[k].cut.get(0);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float a, b;
+                gate_pair(raw[k].g.get(v), a, b);
+                const float from = cut ? 0.f : before[v], xv = raw[k].x.get(v);
+                o[k].A[v] = a;
+                o[k].b[v] = b;
+                o[k].m[v] = (from - xv) * a;
+                const float after = __fmaf_rn(a, from, b * xv);
+                before[v] = on ? after : before[v];
+            }
         }
     }
     __device__ void coef(Item &o, const Raw &i, const Lane &l, const Step &s, bool on) const
     {
+        if constexpr (KEPT) {                                           // (states() has left a, b and m)
+            if (MSK) on = on && s.t() < l.m.len;
+            o.cut = MSK && on && i.cut.get(0);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float a = MSK && o.cut ? 0.f : o.A[v];
+                o.dh[v] = dh.p ? i.dh.get(v) : 0.f;
+                o.S[v] = on && !(MSK && o.cut) ? a * o.dh[v] : 0.f;
+                o.A[v] = on ? a : 1.f;
+            }
+            return;
+        }
         float before[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) before[v] = i.h.get(v);
@@ -261,10 +308,13 @@ template <typename T, int V, bool MSK, typename OFF> struct BackwardOp {
     __device__ void finish(const float (&c)[V], uint32_t ch) const { store_each(dh0, ch, c); }
 };
 
+template <typename T, int V, bool MSK, typename OFF> using BackwardOp = BackwardAnyOp<T, V, MSK, OFF, false>;
+template <typename T, int V, bool MSK, typename OFF> using BackwardKeptOp = BackwardAnyOp<T, V, MSK, OFF, true>;
+
 // 200 x 122880: 76 us for 395 MB (5.2 TB/s, bound by HBM).
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.
 template <int V, bool MSK, bool MOM> struct AdvantageOp {
-    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK, KEEPS = false;
+    static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK, KEEPS = false, BLOCK = false;
     const float *rewards, *values;
     int64_t rew_st, val_st, done_st;
     const uint8_t *dones;
@@ -288,6 +338,7 @@ template <int V, bool MSK, bool MOM> struct AdvantageOp {
         }
         return l;
     }
+    AdvantageOp composing() const { return *this; }
     __device__ void carry0(float (&c)[V], int64_t) const
     {
 #pragma unroll
@@ -373,6 +424,8 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
     const typename Op::Lane ln = op.lane(q, w);
     const int lo = split * q.Ts, hi = lo + q.Ts < q.T ? lo + q.Ts : q.T;
     typename Op::Raw raw[L];
+    float state[V];                                                     // BLOCK: the state in front of this wave's steps
+    static_assert(!Op::BLOCK || L == 8, "states are kept in front of every eighth step");
     auto step_at = [&](int u0, int l) __attribute__((always_inline)) { return Op::REVERSE ? Step{q.T - 1 - u0, -l} : Step{u0, l}; };
     // CLAMP: a step beyond the end reads the last one again, and is not used
     auto load_tile = [&](auto clamp, int tile) __attribute__((always_inline)) {
@@ -382,6 +435,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
             if (decltype(clamp)::value) op.load(raw[l], ln, step_at(u0 + l < hi ? u0 + l : hi - 1, 0), AGG);
             else op.load(raw[l], ln, step_at(u0, l), AGG);
         }
+        if constexpr (Op::BLOCK) op.load_state(state, q, u0, w.ch);
     };
     if (lo < hi) load_tile(std::true_type{}, lo);
     float CA[V], c[V];                                                  // AGG: (CA, c) is the composition so far; else c is the state
@@ -436,6 +490,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
         bool any[V];
 #pragma unroll
         for (int v = 0; v < V; ++v) { PA[v] = 1.f; PS[v] = 0.f; any[v] = false; mine[v] = c[v]; }
+        if constexpr (Op::BLOCK) op.states(it, raw, state, ln, q.T - 1 - u0, FULL ? L : hi - u0);
 #pragma unroll
         for (int l = 0; l < L; ++l) {
             op.coef(it[l], raw[l], ln, step_at(u0, l), FULL || u0 + l < hi);
@@ -476,15 +531,21 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
                 CA[v] = joined<CUTS>(A, CA[v]);
             }
         }
-        if constexpr (!AGG && NW == 1 && Op::KEEPS) {
-            if (op.ck && have && u0 % 8 == 0) store_vec<float, V>(op.ck, (int64_t)(u0 / 8) * q.C + w.ch, c);
-        }
         if (!AGG) {
+            const int kept = (q.T - u0) & 7;                            // the step of these, if any, in front of which the state is kept
+            float front[V];
 #pragma unroll
             for (int l = 0; l < L; ++l) {
                 const bool on = have && (FULL || u0 + l < hi);
+                if constexpr (Op::KEEPS) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) front[v] = l == 0 || l == kept ? mine[v] : front[v];
+                }
                 if constexpr (Op::SUMS) op.step(mine, it[l], ln, step_at(u0, l), on, s1, s2, cnt);
                 else op.step(mine, it[l], ln, step_at(u0, l), on);
+            }
+            if constexpr (Op::KEEPS) {
+                if (op.ck && have && kept < L && u0 + kept < hi) store_vec<float, V>(op.ck, (int64_t)((q.T - u0) / 8 - 1) * q.C + w.ch, front);
             }
             if (NW == 1) {
 #pragma unroll
@@ -519,14 +580,13 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
     }
 }
 
-// The backward pass of many channels, one wave for all of time, from the states that the forward pass kept in front of every eighth step:
-// the eight states in between are computed again, in float32, from the gates and inputs the pass reads anyway, so it reads
-// gate, x, dh and an eighth of a state instead of gate, x, dh and h (200 x 1920 x 256 float32: 384 us for 2.0 GB, 460 us with h).
+// The backward pass of many channels, one wave for all of time, from the states that the forward pass kept: it reads gate, x, dh
+// and an eighth of a state instead of gate, x, dh and h (200 x 1920 x 256 float32: 384 us for 2.0 GB, 460 us with h).
 template <typename T, int V, bool MSK>
-__global__ __launch_bounds__(64) void k_scan_back_kept(BackwardOp<T, V, MSK, uint32_t> op, ScanGeom q, const float *ck)
+__global__ __launch_bounds__(64) void k_scan_back_kept(BackwardKeptOp<T, V, MSK, uint32_t> op, ScanGeom q)
 {
     constexpr int L = 8;
-    typedef BackwardOp<T, V, MSK, uint32_t> Op;
+    typedef BackwardKeptOp<T, V, MSK, uint32_t> Op;
     const uint32_t first = blockIdx.x * 64u * V, mine_ch = first + threadIdx.x * V;
     const bool have = mine_ch < q.C;
     Place w;
@@ -539,27 +599,30 @@ __global__ __launch_bounds__(64) void k_scan_back_kept(BackwardOp<T, V, MSK, uin
     struct Raw { Words<T, V> g, x, dh; Words<uint8_t, 1> cut; };
     Raw raw[L];
     float state[V], c[V];
+    // the block of steps t0 .. t0 + 7; CLAMP: one that begins in front of the first step reads that one again
     auto load = [&](auto clamp, int t0) __attribute__((always_inline)) {
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-            const Step s = decltype(clamp)::value ? Step{t0 + l < q.T ? t0 + l : q.T - 1, 0} : Step{t0, l};
+            const Step s = decltype(clamp)::value ? Step{t0 + l > 0 ? t0 + l : 0, 0} : Step{t0, l};
             fetch(raw[l].g, ln.g, step_off(s, op.gate.st), ln.og);
             fetch(raw[l].x, ln.x, step_off(s, op.x.st), ln.ox);
             if (op.dh.p) fetch(raw[l].dh, ln.dh, step_off(s, op.dh.st), ln.odh);
             if (MSK) { raw[l].cut.w = 0; if (op.marks.resets) fetch(raw[l].cut, ln.r, step_off(s, op.marks.r_st), ln.m.r); }
         }
-        load_vec<float, V>(state, ck, (int64_t)(t0 / L) * q.C + w.ch);
+        op.load_state(state, q, q.T - L - t0, w.ch);
     };
     op.carry0(c, w.ch);
+    // FULL: all eight steps are there.  NEXT: the block in front of this one is 0 none, 1 perhaps not full, 2 full
     auto work = [&](auto full, auto next, int t0) __attribute__((always_inline)) {
-        constexpr bool FULL = decltype(full)::value, NEXT = decltype(next)::value;
+        constexpr bool FULL = decltype(full)::value;
+        constexpr int NEXT = decltype(next)::value;
         float a[L][V], b[L][V], m[L][V], dh[L][V], h[V];
         bool cut[L];
 #pragma unroll
         for (int v = 0; v < V; ++v) h[v] = state[v];
 #pragma unroll
         for (int l = 0; l < L; ++l) {
-            const bool on = (FULL || t0 + l < q.T) && (!MSK || t0 + l < ln.m.len);
+            const bool on = (FULL || t0 + l >= 0) && (!MSK || t0 + l < ln.m.len);
             cut[l] = MSK && raw[l].cut.get(0);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -571,10 +634,10 @@ __global__ __launch_bounds__(64) void k_scan_back_kept(BackwardOp<T, V, MSK, uin
                 h[v] = on ? after : h[v];
             }
         }
-        if constexpr (NEXT) load(std::false_type{}, t0 - L);
+        if constexpr (NEXT != 0) load(std::bool_constant<NEXT == 1>{}, t0 - L);
 #pragma unroll
         for (int l = L - 1; l >= 0; --l) {
-            const bool in = (FULL || t0 + l < q.T), on = in && (!MSK || t0 + l < ln.m.len);
+            const bool in = FULL || t0 + l >= 0, on = in && (!MSK || t0 + l < ln.m.len);
             float og[V], ox[V];
 #pragma unroll
             for (int v = 0; v < V; ++v) {
@@ -589,11 +652,11 @@ __global__ __launch_bounds__(64) void k_scan_back_kept(BackwardOp<T, V, MSK, uin
             }
         }
     };
-    int t0 = (q.T - 1) / L * L;
+    int t0 = q.T - L;
     load(std::true_type{}, t0);
-    if (t0 > 0) { work(std::false_type{}, std::true_type{}, t0); t0 -= L; }
-    for (; t0 > 0; t0 -= L) work(std::true_type{}, std::true_type{}, t0);
-    work(std::false_type{}, std::false_type{}, 0);
+    for (; t0 >= L; t0 -= L) work(std::true_type{}, std::integral_constant<int, 2>{}, t0);
+    if (t0 > 0) { work(std::true_type{}, std::integral_constant<int, 1>{}, t0); t0 -= L; }
+    work(std::false_type{}, std::integral_constant<int, 0>{}, t0);
     if (have) op.finish(c, w.ch);
 }
 

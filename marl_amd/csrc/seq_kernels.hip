@@ -70,7 +70,8 @@ template <int V, int NW, int L, class O> int scan_go(const O &op, const ScanGeom
     const unsigned groups = (unsigned)((q.C + 64 * V - 1) / (64 * V));
     if constexpr (V == 1 && NW == 4)
         if (q.nsplit > 1) {
-            hipLaunchKernelGGL((k_scan<O, V, NW, L, true>), dim3(groups, q.nsplit - 1), dim3(64 * NW), 0, st, op, q, (double *)nullptr);
+            const auto agg = op.composing();
+            hipLaunchKernelGGL((k_scan<std::remove_const_t<decltype(agg)>, V, NW, L, true>), dim3(groups, q.nsplit - 1), dim3(64 * NW), 0, st, agg, q, (double *)nullptr);
             LAUNCH_CHECK();
         }
     hipLaunchKernelGGL((k_scan<O, V, NW, L, false>), dim3(groups, q.nsplit), dim3(64 * NW), 0, st, op, q, mom);
@@ -80,8 +81,10 @@ template <int V, int NW, int L, class O> int scan_go(const O &op, const ScanGeom
 template <template <typename, int, bool, typename> class Op, typename T, bool MSK, class Fill>
 int scan_typed(const Plan &p, bool far, const ScanGeom &q, Fill fill, hipStream_t st)
 {
-    if (p.V == 4) { Op<T, 4, MSK, uint32_t> op; fill(op); return scan_go<4, 1, 4>(op, q, nullptr, st); }
-    if (p.V == 2) { Op<T, 2, MSK, uint32_t> op; fill(op); return scan_go<2, 4, 4>(op, q, nullptr, st); }
+    constexpr bool BLOCK = Op<T, 1, MSK, uint32_t>::BLOCK;
+    if constexpr (!BLOCK)                                               // (with kept states: back_kept())
+        if (p.V == 4) { Op<T, 4, MSK, uint32_t> op; fill(op); return scan_go<4, 1, 4>(op, q, nullptr, st); }
+    if (p.V == 2) { Op<T, 2, MSK, uint32_t> op; fill(op); return scan_go<2, 4, BLOCK ? 8 : 4>(op, q, nullptr, st); }
     if (far) { Op<T, 1, MSK, int64_t> op; fill(op); return p.NW == 8 ? scan_go<1, 8, 8>(op, q, nullptr, st) : scan_go<1, 4, 8>(op, q, nullptr, st); }
     Op<T, 1, MSK, uint32_t> op;
     fill(op);
@@ -114,10 +117,11 @@ int64_t scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
     return n > 1 ? (int64_t)n * 2 * B * D * 4 : 0;
 }
 
-// Bytes of the states a forward pass keeps for its backward pass, 0 where the pass reads h instead.
+// Bytes of the states a forward pass keeps for its backward pass, 0 where the pass reads h instead: bfloat16 for the
+// gradient's sake, float32 for speed.
 int64_t scan_kept(int dtype, int64_t T, int64_t B, int64_t D)
 {
-    return D % 4 == 0 && scan_plan(T, B * D, dtype ? 2 : 4, true, true).NW == 1 ? (T + 7) / 8 * B * D * 4 : 0;
+    return dtype || (D % 4 == 0 && scan_plan(T, B * D, 4, true, true).NW == 1) ? (T + 7) / 8 * B * D * 4 : 0;
 }
 
 static ScanGeom scan_geom(const ScanArgs &a, const Plan &p)
@@ -136,7 +140,7 @@ int launch_scan_forward(const ScanArgs &a, hipStream_t st)
     };
     const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
     return scan_dispatch<ForwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
-        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last; op.ck = a.kept;
+        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last; op.ck = a.dtype || p.NW == 1 ? a.kept : nullptr;
         op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
     }, st);
 }
@@ -144,14 +148,14 @@ int launch_scan_forward(const ScanArgs &a, hipStream_t st)
 template <class Op> static void fill_backward(Op &op, const ScanArgs &a)
 {
     op.gate = a.gate; op.x = a.x; op.h = a.h; op.dh = a.dh; op.dgate = a.dgate; op.dx = a.dx;
-    op.h0 = a.h0; op.dh_last = a.dh_last; op.dh0 = a.dh0;
+    op.h0 = a.h0; op.dh_last = a.dh_last; op.dh0 = a.dh0; op.ck = a.kept;
     op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
 }
 template <typename T, bool MSK> static int back_kept(const ScanArgs &a, const ScanGeom &q, hipStream_t st)
 {
-    BackwardOp<T, 4, MSK, uint32_t> op;
+    BackwardKeptOp<T, 4, MSK, uint32_t> op;
     fill_backward(op, a);
-    hipLaunchKernelGGL((k_scan_back_kept<T, 4, MSK>), dim3((q.C + 255) / 256), dim3(64), 0, st, op, q, a.kept);
+    hipLaunchKernelGGL((k_scan_back_kept<T, 4, MSK>), dim3((q.C + 255) / 256), dim3(64), 0, st, op, q);
     LAUNCH_CHECK();
     return 0;
 }
@@ -172,7 +176,11 @@ int launch_scan_backward(const ScanArgs &a, hipStream_t st)
         if (a.dtype == 0) return msk ? back_kept<float, true>(a, scan_geom(a, p), st) : back_kept<float, false>(a, scan_geom(a, p), st);
         return msk ? back_kept<bf16, true>(a, scan_geom(a, p), st) : back_kept<bf16, false>(a, scan_geom(a, p), st);
     }
-    return scan_dispatch<BackwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) { fill_backward(op, a); }, st);
+    const bool msk = a.resets || a.lengths;
+    const auto fill = [&](auto &op) { fill_backward(op, a); };
+    if (a.dtype && a.kept && a.T > 0)
+        return msk ? scan_typed<BackwardKeptOp, bf16, true>(p, far, scan_geom(a, p), fill, st) : scan_typed<BackwardKeptOp, bf16, false>(p, far, scan_geom(a, p), fill, st);
+    return scan_dispatch<BackwardOp>(a.dtype, msk, p, far, scan_geom(a, p), fill, st);
 }
 
 int launch_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb, float *state,
