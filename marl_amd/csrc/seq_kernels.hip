@@ -140,7 +140,7 @@ int launch_scan_forward(const ScanArgs &a, hipStream_t st)
     };
     const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
     return scan_dispatch<ForwardOp>(a.dtype, a.resets || a.lengths, p, far, scan_geom(a, p), [&](auto &op) {
-        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last; op.ck = a.dtype || p.NW == 1 ? a.kept : nullptr;
+        op.gate = a.gate; op.x = a.x; op.out = a.out; op.h0 = a.h0; op.h_last = a.h_last; op.ck = a.kept;
         op.marks = Marks{a.lengths, a.resets, a.r_st, a.r_sb};
     }, st);
 }
@@ -170,13 +170,12 @@ int launch_scan_backward(const ScanArgs &a, hipStream_t st)
                vec_ok(a.dh.p, a.dh.st, a.dh.sb, e, V) && vec_ok(a.dgate.p, a.dgate.st, a.dgate.sb, e, V) && vec_ok(a.dx.p, a.dx.st, a.dx.sb, e, V);
     };
     const Plan p = scan_plan(a.T, a.B * a.D, e, rows(2), rows(4));
-    // (whatever lets this pass go four channels a lane let the forward pass, which then kept its states)
+    // (the forward pass leaves its states however its own tensors were aligned: these here may be copies of them)
+    const bool msk = a.resets || a.lengths;
     if (p.NW == 1 && a.kept && a.T > 0) {
-        const bool msk = a.resets || a.lengths;
         if (a.dtype == 0) return msk ? back_kept<float, true>(a, scan_geom(a, p), st) : back_kept<float, false>(a, scan_geom(a, p), st);
         return msk ? back_kept<bf16, true>(a, scan_geom(a, p), st) : back_kept<bf16, false>(a, scan_geom(a, p), st);
     }
-    const bool msk = a.resets || a.lengths;
     const auto fill = [&](auto &op) { fill_backward(op, a); };
     if (a.dtype && a.kept && a.T > 0)
         return msk ? scan_typed<BackwardKeptOp, bf16, true>(p, far, scan_geom(a, p), fill, st) : scan_typed<BackwardKeptOp, bf16, false>(p, far, scan_geom(a, p), fill, st);
