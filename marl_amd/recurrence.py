@@ -129,6 +129,7 @@ class _GatedScan(torch.autograd.Function):
     def backward(ctx, dh, dlast):
         _once("gated_scan")
         gate, x, h, h0, resets, lengths, kept = ctx.saved_tensors
+        gate, x, h = _dense(gate), _dense(x), _dense(h)                  # (saved-tensor hooks may hand back other strides)
         T, B, D = ctx.dims
         bf, dev, dt = ctx.batch_first, gate.device, _DTYPES[gate.dtype]
         dh = None if dh is None else _dense(dh)

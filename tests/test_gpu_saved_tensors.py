@@ -27,3 +27,17 @@ def test_saved_tensors_may_come_back_dense(torch_cuda, T, B, D, dtype):
         want = _want(gate, x, None, None, None, False, dh, dl)
         for name, got in zip(("h", "last", "dgate", "dx"), (h, last) + grads):
             so.within(got, *want[name], f"offset {lo} {name}")
+
+
+def test_saved_tensors_may_come_back_transposed(torch_cuda):
+    torch = torch_cuda
+    from marl_amd.recurrence import gated_scan
+    T, B, D = 9, 4, 6
+    leaves = [torch.randn(T, B, D, device="cuda", requires_grad=True) for _ in range(2)]
+    turned = lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() == 3 else t  # noqa: E731
+    with torch.autograd.graph.saved_tensors_hooks(turned, lambda t: t):
+        h, last = gated_scan(*leaves)
+    dh, dl = torch.randn_like(h), torch.randn_like(last)
+    got = torch.autograd.grad((h, last), leaves, (dh, dl))
+    want = torch.autograd.grad(gated_scan(*leaves), leaves, (dh, dl))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
