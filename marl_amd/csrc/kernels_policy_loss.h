@@ -7,11 +7,10 @@
 //   loss = mean of L_r over the rows the mask leaves (no rows: 0, and so are the gradients)
 //   dL_r / dlog_pi = (cut ? 0 : -q A) - kl (e^D - 1),   cut = A > 0 and q > 1 + eps, or A < 0 and q < 1 - eps
 //   dmu_j = dL/dlog_pi z_j e^-s_j,      ds_j = dL/dlog_pi (z_j^2 - 1) - ent
-// What is in double and what is not: z, log_pi, d and q = e^d are in double, and so is the decision whether a ratio lies beyond the
-// clipping border (d against log(1 +- eps): it decides between a gradient and none) and the sum of the gains, whose terms
-// cancel.  e^D - 1 - D, which cancels for nearly equal policies, is its own series where |D| < 1, in float32; so are the
-// products behind the row's gradient.  Sums are in double.  Measured at 24.6 M rows of two components: 167 us for 787 MB, 4.7 TB/s (a copy of
-// 2 GiB reaches 4.95), 180 vector instructions a row, 0.55 of the issue; every row wholly in double: 189 us, bound by its instructions.
+// A row is wholly in double and rounded once, where it is stored: d against log(1 +- eps) decides between a gradient and none, the
+// terms of the gains cancel, and e^D - 1 - D does for nearly equal policies; q and e^D have the range of double (one row whose action the
+// policy of now finds very unlikely must not take the others with it), and without a KL term in the loss e^D does not enter
+// it at all.  Measured at 24.6 M rows of two components: 171 us for 787 MB, 4.6 TB/s (a copy of 2 GiB reaches 4.95).
 // 2048 rows in one workgroup: 9 us, its two trips to memory and one long chain of dependent double operations a row.
 // The gradients are written in the same pass as the loss: a mean over rows needs only their count, known without a mask
 // and counted ahead with one.  Sums: per thread, per workgroup in a fixed order, then over the workgroups in a fixed order:
@@ -79,49 +78,35 @@ template <typename TM, bool SHARED> __device__ __forceinline__ void loss_finish(
     if (threadIdx.x == 0) {
         const double inv = 1.0 / (double)(count > 0 ? count : 1);
         const double gain = tot[0] * inv, kl = tot[1] * inv, ent = tot[2] * inv;
-        p.loss[0] = (float)(-gain + p.kl * kl - p.ent * ent);
+        p.loss[0] = (float)(-gain + (p.kl != 0.0 ? p.kl * kl : 0.0) - p.ent * ent);
         p.stats[0] = (float)gain; p.stats[1] = (float)kl; p.stats[2] = (float)ent;
         p.stats[3] = (float)(tot[3] * inv); p.stats[4] = (float)(tot[4] * inv); p.stats[5] = (float)count;
     }
     if (SHARED && threadIdx.x < (unsigned)p.A) reinterpret_cast<TM *>(p.dstd)[threadIdx.x] = from_float<TM>((float)tot[LOSS_SUMS + threadIdx.x]);
 }
 
-// e^x and e^-x in double for |x| < 700 (beyond: infinite or 0): x = n log 2 + r, |r| <= log(2) / 2, the even and the odd part of
-// e^r's series up to r^13 (the next term is below 1e-17), their sum and difference scaled by 2^n and 2^-n.
-__device__ __forceinline__ void exp_both(double x, double &ep, double &em)
+// q = e^d, em = e^-d - 1 and k = e^-d - 1 + d, in double: d = n log 2 + r with |r| <= log(2) / 2 (the two-part log 2 of fdlibm's
+// e_exp.c, whose first part times n is exact), the even part 1 + E and the odd part r + O of e^r's series up to r^13 (the next term
+// is below 1e-17), their sum and difference scaled by 2^n and 2^-n.  em and k come from E and O where n = 0, without a
+// cancellation; beyond, |d| > 0.34 and e^-d - 1 + d loses at most a factor (e^-d + 1 + |d|) / k < 50 of its last place.  |d| > 745:
+// infinite or 0.  NaN stays.
+__device__ __forceinline__ void exp_parts(double d, double &q, double &em, double &k)
 {
-    const double c = x > 800.0 ? 800.0 : x < -800.0 ? -800.0 : x;       // (NaN stays)
+    const double c = d > 800.0 ? 800.0 : d < -800.0 ? -800.0 : d;
     const double n = __builtin_rint(c * 1.44269504088896340736), r = __fma_rn(n, -1.9082149292705877e-10, __fma_rn(n, -0.69314718036912381649, c)), s = r * r;
-    double e = 1.0 / 479001600.0, o = 1.0 / 6227020800.0;
-    e = __fma_rn(e, s, 1.0 / 3628800.0); o = __fma_rn(o, s, 1.0 / 39916800.0);
-    e = __fma_rn(e, s, 1.0 / 40320.0);   o = __fma_rn(o, s, 1.0 / 362880.0);
-    e = __fma_rn(e, s, 1.0 / 720.0);     o = __fma_rn(o, s, 1.0 / 5040.0);
-    e = __fma_rn(e, s, 1.0 / 24.0);      o = __fma_rn(o, s, 1.0 / 120.0);
-    e = __fma_rn(e, s, 0.5);             o = __fma_rn(o, s, 1.0 / 6.0);
-    e = __fma_rn(e, s, 1.0);             o = __fma_rn(o, s, 1.0) * r;
-    const int k = (int)n;
-    ep = __builtin_ldexp(e + o, k);
-    em = __builtin_ldexp(e - o, -k);
-}
-
-// k = e^x - 1 - x and em = e^x - 1, e = e^x given.  |x| < 1: x^2 (1/2! + x/3! + ... + x^9/11!), the rest below 2^-28 of it;
-// beyond, e^x - 1 - x loses at most a factor (e + 1 + |x|) / k < 8 of the rounding.
-__device__ __forceinline__ void expm1_parts(float x, float e, float &k, float &em)
-{
-    float s = 2.5052108385441718775e-8f;                                // 1/11!
-    s = __fmaf_rn(s, x, 2.7557319223985890653e-7f);
-    s = __fmaf_rn(s, x, 2.7557319223985892511e-6f);
-    s = __fmaf_rn(s, x, 2.4801587301587301566e-5f);
-    s = __fmaf_rn(s, x, 1.9841269841269841253e-4f);
-    s = __fmaf_rn(s, x, 1.3888888888888889419e-3f);
-    s = __fmaf_rn(s, x, 8.3333333333333332177e-3f);
-    s = __fmaf_rn(s, x, 4.1666666666666664354e-2f);
-    s = __fmaf_rn(s, x, 1.6666666666666665741e-1f);
-    s = __fmaf_rn(s, x, 0.5f);
-    const float small = s * x * x;
-    const bool near = fabsf(x) < 1.f;
-    em = near ? x + small : e - 1.f;
-    k = near ? small : em - x;
+    double E = 1.0 / 479001600.0, O = 1.0 / 6227020800.0;
+    E = __fma_rn(E, s, 1.0 / 3628800.0); O = __fma_rn(O, s, 1.0 / 39916800.0);
+    E = __fma_rn(E, s, 1.0 / 40320.0);   O = __fma_rn(O, s, 1.0 / 362880.0);
+    E = __fma_rn(E, s, 1.0 / 720.0);     O = __fma_rn(O, s, 1.0 / 5040.0);
+    E = __fma_rn(E, s, 1.0 / 24.0);      O = __fma_rn(O, s, 1.0 / 120.0);
+    E = __fma_rn(E, s, 0.5) * s;         O = __fma_rn(O, s, 1.0 / 6.0) * (s * r);
+    const double e = 1.0 + E, o = r + O;
+    const int i = (int)n;
+    q = __builtin_ldexp(e + o, i);
+    const double inv = __builtin_ldexp(e - o, -i);
+    const bool near = n == 0.0;
+    em = near ? E - o : inv - 1.0;
+    k = near ? E - O : em + d;
 }
 
 // A row is worked on by GL neighbouring lanes, AM components each (lane `sub` of them has components sub AM .. sub AM + AM - 1):
@@ -155,7 +140,7 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
     }
     __syncthreads();
     const double wd = 1.0 / (double)(count > 0 ? count : 1);
-    const float w = (float)wd, klf = (float)p.kl, entw = (float)(p.ent * wd);
+    const double entw = p.ent * wd;
     double am = 0.0, ar = 1.0;
     if (p.moments) { am = (double)p.moments[0]; ar = (double)p.moments[1]; }
     double sum[LOSS_SUMS + AM];
@@ -223,63 +208,61 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
         if (base + ROWS + lane_row < last) { move_on(); fetch_row(nxt, base + ROWS); }
         const bool valid = have && (!masked || cur.ok != 0);
         const double adv = ((double)cur.adv - am) * ar;
-        float zf[AM], ef[AM];
+        double z[AM], es[AM];                                           // (es: e^-s)
         double lp = 0.0, ent = 0.0;
 #pragma unroll
         for (int j = 0; j < AM; ++j) {
             if (LINEAR || j0 + j < p.A) {
-                const double s = SHARED ? sh_s[j0 + j] : (double)to_float(cur.sd.v[j]), e = SHARED ? sh_e[j0 + j] : exp(-s);
-                const double z = ((double)cur.u[j] - (double)to_float(cur.mu.v[j])) * e;
-                lp = __fma_rn(-0.5 * z, z, lp - (s + 0.91893853320467274178));        // log(2 pi) / 2
+                const double s = SHARED ? sh_s[j0 + j] : (double)to_float(cur.sd.v[j]);
+                es[j] = SHARED ? sh_e[j0 + j] : exp(-s);
+                z[j] = ((double)cur.u[j] - (double)to_float(cur.mu.v[j])) * es[j];
+                lp = __fma_rn(-0.5 * z[j], z[j], lp - (s + 0.91893853320467274178));  // log(2 pi) / 2
                 ent += s;
-                zf[j] = (float)z; ef[j] = (float)e;
             }
         }
 #pragma unroll
         for (int o = GL / 2; o; o >>= 1) { lp += __shfl_xor(lp, o, 64); ent += __shfl_xor(ent, o, 64); }
         const double d = lp - (double)cur.old;
-        double q, eD;
-        exp_both(d, q, eD);                                             // (without a reference of its own, D = -d)
-        float D = (float)-d, k3, em;
+        double q, em, k3;
+        exp_parts(d, q, em, k3);                                        // (without a reference of its own, D = -d)
         if (own_ref) {
-            const double Dd = (double)cur.ref - lp;
             double unused;
-            exp_both(Dd, eD, unused);
-            D = (float)Dd;
+            exp_parts(lp - (double)cur.ref, unused, em, k3);
         }
-        expm1_parts(D, (float)eD, k3, em);
         const bool above = d > p.dhi, below = d < p.dlo, cut = (adv > 0.0 && above) || (adv < 0.0 && below);
         const double qa = q * adv;
-        const float g = w * ((cut ? 0.f : -(float)qa) - klf * em);
+        const double g = wd * ((cut ? 0.0 : -qa) - (p.kl != 0.0 ? p.kl * em : 0.0));      // (em may be infinite: no term, no trace of it)
         if (valid && sub == 0) {
             sum[0] += cut ? (above ? p.hi : p.lo) * adv : qa;            // min(q A, clip(q) A): the clipped one where it cuts
-            sum[1] += (double)k3;
+            sum[1] += k3;
             sum[2] += ent + p.A * 1.41893853320467274178;               // (log(2 pi) + 1) / 2
             sum[3] += cut ? 1.0 : 0.0;
             sum[4] += q;
         }
-        float dm[AM], ds[AM];
+        float dm[AM], dsf[AM];
 #pragma unroll
         for (int j = 0; j < AM; ++j) {
-            dm[j] = 0.f; ds[j] = 0.f;
+            double ds = 0.0;
+            dm[j] = 0.f;
             if ((LINEAR || j0 + j < p.A) && valid) {
-                dm[j] = g * zf[j] * ef[j];
-                ds[j] = __fmaf_rn(g, __fmaf_rn(zf[j], zf[j], -1.f), -entw);
+                dm[j] = (float)(g * z[j] * es[j]);
+                ds = __fma_rn(g, __fma_rn(z[j], z[j], -1.0), -entw);
             }
-            if constexpr (SHARED) sum[LOSS_SUMS + j] += (double)ds[j];
+            if constexpr (SHARED) sum[LOSS_SUMS + j] += ds;
+            dsf[j] = (float)ds;
         }
         if (have) {
             if (LINEAR) {
                 char *pd = reinterpret_cast<char *>(p.dmean) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM));
                 put<TM, AM>(pd, 0, (uint32_t)(tid * AM * sizeof(TM)), dm);
-                if (!SHARED) put<TM, AM>(reinterpret_cast<char *>(p.dstd) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM)), 0, (uint32_t)(tid * AM * sizeof(TM)), ds);
+                if (!SHARED) put<TM, AM>(reinterpret_cast<char *>(p.dstd) + (int64_t)base * (int64_t)(AM * GL * sizeof(TM)), 0, (uint32_t)(tid * AM * sizeof(TM)), dsf);
             } else {
                 const int64_t at = (int64_t)(base + lane_row) * p.A + j0;
 #pragma unroll
                 for (int j = 0; j < AM; ++j)
                     if (j0 + j < p.A) {
                         reinterpret_cast<TM *>(p.dmean)[at + j] = from_float<TM>(dm[j]);
-                        if (!SHARED) reinterpret_cast<TM *>(p.dstd)[at + j] = from_float<TM>(ds[j]);
+                        if (!SHARED) reinterpret_cast<TM *>(p.dstd)[at + j] = from_float<TM>(dsf[j]);
                     }
             }
         }
