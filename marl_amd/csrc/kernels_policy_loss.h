@@ -20,7 +20,7 @@ constexpr int LOSS_SUMS = 5;                                            // gain,
 
 struct LossDev {
     uint32_t rows, n, B;
-    int A;
+    int A, own_ref;                                                     // own_ref: ref is not old
     Rows mean, log_std, actions, old, ref, adv, mask;
     const float *moments;
     double lo, hi, dlo, dhi, kl, ent;                                   // 1 -+ clip and their logarithms
@@ -122,7 +122,7 @@ __global__ __launch_bounds__(BS) void k_policy_loss(LossDev p)
     __shared__ double sh_s[AM * GL], sh_e[AM * GL], red[BS / 64][K], tot[K];
     __shared__ int64_t sh_c[BS / 64];
     const int tid = threadIdx.x, sub = GL > 1 ? tid & (GL - 1) : 0, j0 = sub * AM;
-    const bool masked = p.mask.p != nullptr, own_ref = p.ref.p != p.old.p;
+    const bool masked = p.mask.p != nullptr, own_ref = p.own_ref;
     const uint8_t *maskp = reinterpret_cast<const uint8_t *>(p.mask.p);
     if (SHARED && tid < p.A) {
         const double s = (double)to_float(reinterpret_cast<const TM *>(p.log_std.p)[tid * p.log_std.sa]);

@@ -300,6 +300,7 @@ int launch_policy_loss(const LossArgs &a, hipStream_t st)
     p.rows = (uint32_t)(a.B * a.n); p.n = (uint32_t)std::max<int64_t>(a.n, 1); p.B = (uint32_t)a.B; p.A = a.A;
     p.mean = a.mean; p.log_std = a.log_std; p.actions = a.actions; p.old = a.log_pi_old;
     p.ref = a.log_pi_ref.p ? a.log_pi_ref : a.log_pi_old;
+    p.own_ref = p.ref.p != p.old.p || p.ref.sb != p.old.sb || p.ref.sn != p.old.sn;
     p.adv = a.adv; p.mask = a.mask; p.moments = a.adv_moments;
     p.dlo = a.clip < 1.0 ? std::log1p(-a.clip) : -INFINITY; p.dhi = std::log1p(a.clip);       // (a ratio is never below 0)
     p.lo = 1.0 - a.clip; p.hi = 1.0 + a.clip; p.kl = a.kl_coef; p.ent = a.entropy_coef;

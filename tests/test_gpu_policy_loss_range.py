@@ -127,3 +127,20 @@ def test_precision_of_whole_episodes(torch_cuda):
     _same(torch, loss, *wl, torch.float32, "loss")
     _same(torch, dm, *wm, torch.float32, "dmean")
     _same(torch, ds, *ws, torch.float32, "dlog_std")
+
+
+def test_a_reference_that_begins_where_the_old_policy_does(torch_cuda):
+    """Two views of one buffer that begin at the same element are still two tensors."""
+    torch = torch_cuda
+    from marl_amd.policy_loss import clipped_policy_loss
+    for lead in ((50,), (6000,), (40, 30)):
+        N = math.prod(lead)
+        mean, std = torch.zeros(*lead, 1, device="cuda"), torch.zeros(1, device="cuda")
+        act, adv = torch.randn(*lead, 1, device="cuda"), torch.randn(lead, device="cuda")
+        rows = so.log_pi(mean, std, act).float().cuda() + 0.2 * torch.randn(lead, device="cuda")
+        rows.view(-1)[0] = -1.0
+        one = rows.view(-1)[:1].expand(N).view(lead) if len(lead) == 1 else rows[:1, :1].expand(lead)
+        for old, ref in ((one, rows), (rows, one)):
+            got = clipped_policy_loss(mean, std, act, old, adv, log_pi_ref=ref, kl_coef=0.3)
+            want = clipped_policy_loss(mean, std, act, old.clone(), adv, log_pi_ref=ref.clone(), kl_coef=0.3)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), lead
