@@ -735,8 +735,11 @@ int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, cons
 
 int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream)
 {
-    if (int rc = seq_dims("asm_policy_loss_scale", dtype, 1, n_mean, 1)) return rc;
-    if (n_std < 0 || !grad || (n_mean > 0 && !dmean) || (n_std > 0 && !dlog_std)) return fail(1, "asm_policy_loss_scale: bad arguments");
+    if (int rc = seq_dims("asm_policy_loss_scale", dtype, 1, 1, 1)) return rc;
+    // (numbers of values: 32 of each row that asm_policy_loss takes)
+    if (n_mean < 0 || n_std < 0 || n_mean > (INT64_C(32) << 29) || n_std > (INT64_C(32) << 29))
+        return fail(1, "asm_policy_loss_scale: %lld and %lld values: negative or too large", (long long)n_mean, (long long)n_std);
+    if (!grad || (n_mean > 0 && !dmean) || (n_std > 0 && !dlog_std)) return fail(1, "asm_policy_loss_scale: bad arguments");
     int rc = asmseq::launch_policy_loss_scale(dtype, grad, n_mean, dmean, n_std, dlog_std, (hipStream_t)stream);
     return rc ? hip_fail(rc, "asm_policy_loss_scale") : 0;
 }

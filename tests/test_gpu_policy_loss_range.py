@@ -144,3 +144,22 @@ def test_a_reference_that_begins_where_the_old_policy_does(torch_cuda):
             got = clipped_policy_loss(mean, std, act, old, adv, log_pi_ref=ref, kl_coef=0.3)
             want = clipped_policy_loss(mean, std, act, old.clone(), adv, log_pi_ref=ref.clone(), kl_coef=0.3)
             assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), lead
+
+
+def test_more_gradient_values_than_2_to_the_29(torch_cuda):
+    """2^28 + 1 rows of two components, all alike (expanded inputs): their gradients, scaled by an upstream gradient of a half."""
+    torch = torch_cuda
+    from marl_amd.policy_loss import clipped_policy_loss
+    N = (1 << 28) + 1
+    m = torch.tensor([[0.1, -0.2]], device="cuda").expand(N, 2).detach().requires_grad_()
+    s = torch.tensor([-0.5, -0.4], device="cuda").requires_grad_()
+    act, one = torch.tensor([[0.3, 0.1]], device="cuda").expand(N, 2), torch.ones(1, device="cuda").expand(N)
+    loss, _ = clipped_policy_loss(m, s, act, -1.5 * one, -one)
+    dm, ds = torch.autograd.grad(loss, (m, s), torch.tensor(0.5, device="cuda"))
+    z = (act[0].cpu().double() - m[0].detach().cpu().double()) * torch.exp(-s.detach().cpu().double())
+    q = torch.exp((-z * z / 2 - s.detach().cpu().double() - math.log(2 * math.pi) / 2).sum() + 1.5)
+    want = 0.5 * q / N * z * torch.exp(-s.detach().cpu().double())      # (q is not clipped: the advantage is negative and q above 1)
+    assert float(q) > 1.0
+    so.within(dm[0], want, 2 * so.U * want.abs(), "dmean")              # two roundings: stored, scaled
+    assert bool((dm == dm[0]).all())
+    so.within(ds, 0.5 * q * (z * z - 1), 2 * so.U * (q * (z * z - 1)).abs() + 1e-9, "dlog_std")
