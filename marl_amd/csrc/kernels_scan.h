@@ -56,15 +56,20 @@ template <int V> __device__ __forceinline__ void store_each(float *p, uint32_t c
     }
 }
 
-// a = sigmoid(g) and b = 1 - a from e = exp(-g): a = 1 / (1 + e), b = e a where e < 1 and 1 - a elsewhere, so neither end
-// loses digits and nothing is infinite times zero.  The exponential and the reciprocal are the hardware's (1 unit in the
-// last place each); what remains is the rounding of g log2(e), |g| units of e: with the sums, a and b are good to 4 + |g|
-// units.  (The correction of that rounding and a Newton step cost 9 of 22 instruction slots an element.)  NaN stays NaN.
+// a = sigmoid(g) and b = 1 - a from t = e^-|g| <= 1: the larger of the two is 1 / (1 + t), the smaller t / (1 + t), so neither end loses
+// digits and nothing overflows.  |g| log2(e) = n + f with |f| <= 1/2, f by two fused products with the two parts of log2(e), so its
+// rounding does not grow with |g|; 2^f and the reciprocal are the hardware's (1 unit in the last place each), the reciprocal
+// with a Newton step.  a and b are good to 6 halves of a unit down to the smallest numbers.  n stops at 160, where t is 0.
+// NaN stays NaN.
 __device__ __forceinline__ void gate_pair(float g, float &a, float &b)
 {
-    const float e = __builtin_amdgcn_exp2f(g * -1.44269504088896340736f);
-    a = __builtin_amdgcn_rcpf(1.0f + e);
-    b = e < 1.0f ? e * a : 1.0f - a;
+    const float y = fabsf(g);
+    const float n = fmaxf(__builtin_rintf(y * -1.44269504088896340736f), -160.0f);
+    const float f = __fmaf_rn(y, -1.92596299112661746887e-8f, __fmaf_rn(y, -1.44269504088896340736f, -n));
+    const float t = __builtin_ldexpf(__builtin_amdgcn_exp2f(f), (int)n), s = 1.0f + t, r = __builtin_amdgcn_rcpf(s);
+    const float big = __fmaf_rn(__fmaf_rn(-s, r, 1.0f), r, r), small = t * big;
+    a = g < 0.0f ? small : big;
+    b = g < 0.0f ? big : small;
 }
 
 struct ScanGeom {
