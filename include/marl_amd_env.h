@@ -434,6 +434,8 @@ int64_t asm_policy_loss_workspace(int64_t rows, int A);
 int asm_policy_loss(int dtype, int64_t B, int64_t n, int A, int shared_std, const asm_loss_rows *rows,
                     const float *adv_moments /*nullable*/, double clip, double kl_coef, double entropy_coef, float *loss, float *stats,
                     void *dmean, void *dlog_std, void *ws, int64_t ws_bytes, void *stream);
+/* Which capture into a HIP graph `stream` is part of: a number of its own for each, 0 for none. */
+uint64_t asm_capture_id(void *stream);
 /* Multiplies n_mean values of dmean and n_std of dlog_std by *grad (device); reads and writes nothing when that is 1. */
 int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream);
 /* actions = mean + e^log_std noise (noise.p NULL: actions are given, not written) and log_pi of the actions as they are

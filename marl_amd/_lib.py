@@ -53,7 +53,7 @@ EXPORTS = ["_get_observation", "_get_reward", "_sf_b2b_all", "_get_dist_b2w", "c
            "asm_policy_mlp_forward_bf16", "asm_policy_mlp_act_bf16", "asm_obs_rows_f32",
            "asm_gated_scan_workspace", "asm_gated_scan_kept", "asm_gated_scan_forward", "asm_gated_scan_backward", "asm_gated_scan_step",
            "asm_advantages_workspace", "asm_advantages_f32", "asm_policy_loss_workspace", "asm_policy_loss",
-           "asm_policy_loss_scale", "asm_gaussian_act"]
+           "asm_policy_loss_scale", "asm_capture_id", "asm_gaussian_act"]
 
 _lib = None
 
@@ -139,6 +139,8 @@ def load() -> C.CDLL:
     lib.asm_policy_loss.argtypes = [i32, i64, i64, i32, i32, vp, vp, f64, f64, f64] + [vp] * 5 + [i64, vp]
     lib.asm_policy_loss_scale.restype = C.c_int
     lib.asm_policy_loss_scale.argtypes = [i32, vp, i64, vp, i64, vp, vp]
+    lib.asm_capture_id.restype = u64
+    lib.asm_capture_id.argtypes = [vp]
     lib.asm_gaussian_act.restype = C.c_int
     lib.asm_gaussian_act.argtypes = [i32, i64, i64, i32, vp, vp]
     lib.asm_set_step_schedule.restype = None

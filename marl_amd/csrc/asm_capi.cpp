@@ -744,6 +744,14 @@ int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dm
     return rc ? hip_fail(rc, "asm_policy_loss_scale") : 0;
 }
 
+uint64_t asm_capture_id(void *stream)
+{
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess || status != hipStreamCaptureStatusActive) return 0;
+    return id;
+}
+
 int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_act_rows *t, void *stream)
 {
     if (int rc = policy_dims("asm_gaussian_act", dtype, B, n, A)) return rc;

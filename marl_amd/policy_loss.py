@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .recurrence import _DTYPES, _FLAGS, _call, _guard_leaves, _need, _on_device, _once, _ptr, _workspace
+from .recurrence import _DTYPES, _FLAGS, _call, _capture, _guard_leaves, _need, _on_device, _once, _ptr, _workspace
 
 STATS_FIELDS = ("gain", "kl", "entropy", "clipped", "ratio", "rows")
 _NO_ROWS = (0, 0, 0, 0)
@@ -99,7 +99,7 @@ class _ClippedLoss(torch.autograd.Function):
     def forward(ctx, mean, log_std, fixed, options):                    # fixed: the tensors without a gradient
         ctx.set_materialize_grads(False)
         loss, stats, dmean, dstd = _loss(mean, log_std, *fixed, *options)
-        ctx.grads, ctx.options = (dmean, dstd), options
+        ctx.grads, ctx.options, ctx.capture = (dmean, dstd), options, _capture(mean.device)
         ctx.save_for_backward(mean, log_std, *fixed)
         ctx.mark_non_differentiable(stats)
         return loss, stats
@@ -109,9 +109,12 @@ class _ClippedLoss(torch.autograd.Function):
         if g is None:
             return None, None, None, None
         _once("clipped_policy_loss")
-        # the gradients of the forward pass are handed out once; a second backward pass over a retained graph makes its own
+        # the gradients of the forward pass are handed out once, scaled where they are; a second backward pass over a retained graph
+        # makes its own, and so does one that is captured apart from the forward pass: its replays would scale them again
         tensors = ctx.saved_tensors                                     # (notices inputs overwritten since)
-        grads, ctx.grads = ctx.grads, None
+        grads = None
+        if ctx.capture == _capture(g.device):
+            grads, ctx.grads = ctx.grads, None
         dmean, dstd = grads if grads is not None else _loss(*tensors, *ctx.options)[2:]
         _call("asm_policy_loss_scale", dmean.device, _DTYPES[dmean.dtype], g.data_ptr(), dmean.numel(), dmean.data_ptr(), dstd.numel(), dstd.data_ptr())
         return dmean, dstd, None, None

@@ -72,6 +72,13 @@ def _once(fn: str) -> None:
         raise RuntimeError(f"{fn} is differentiable once: no create_graph=True through it")
 
 
+def _capture(dev: torch.device) -> int:
+    """The capture into a HIP graph that dev's current stream is part of, 0 for none."""
+    if torch.cuda.current_device() == dev.index and not torch.cuda.is_current_stream_capturing():
+        return 0
+    return _lib.load().asm_capture_id(_raw_stream(dev.index))
+
+
 def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
     """A leaf's accumulation node belongs to the stream it was first used on and lives as long as any graph that uses the
     leaf; a backward pass captured into a HIP graph would have to join that other stream, which ends the process.
