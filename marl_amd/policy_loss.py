@@ -204,6 +204,8 @@ def gaussian_log_pi(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Te
 
 
 def _act(fn, mean, log_std, noise, actions, log_pi):
+    for name, t in (("actions", None if noise is None else actions), ("log_pi", log_pi)):
+        _need(t is None or not (t.requires_grad and torch.is_grad_enabled()), f"{fn}: {name} is written in place and cannot require a gradient")
     if not _policy_ok(mean, log_std, (noise, actions), (log_pi,)):
         _explain_policy(fn, mean, log_std, dict(noise=noise, actions=actions), dict(log_pi=log_pi))
         _on_device(fn, mean.device, log_std, noise, actions, log_pi)
