@@ -195,11 +195,13 @@ def gaussian_act(mean: torch.Tensor, log_std: torch.Tensor, noise: torch.Tensor,
     log-probability of the actions as they are stored in float32, so that a ratio taken from it later starts at 1.
     noise: standard normal draws of mean's shape (torch.randn); log_std: mean's shape, or (A,) for all rows.  actions, log_pi: where to write
     (strided views are fine: DeviceReplay.action_slot().transpose(-1, -2))."""
+    _need(noise is not None, "gaussian_act: noise must be a float32 tensor of mean's shape")
     return _act("gaussian_act", mean, log_std, noise, actions, log_pi)
 
 
 def gaussian_log_pi(mean: torch.Tensor, log_std: torch.Tensor, actions: torch.Tensor, *, log_pi: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Log-probabilities of given actions, without gradients: what a reference policy says of a recorded episode."""
+    _need(actions is not None, "gaussian_log_pi: actions must be a float32 tensor of mean's shape")
     return _act("gaussian_log_pi", mean, log_std, None, actions, log_pi)[1]
 
 

@@ -28,3 +28,13 @@ def test_outputs_that_require_a_gradient(call):
 def test_given_actions_may_require_one():
     with pytest.raises(ValueError, match="HIP device"):
         gaussian_log_pi(_grad(5, 2), S, _grad(5, 2))
+
+
+def test_no_noise_and_no_actions():
+    """(an uninitialised tensor was taken in their place)"""
+    with pytest.raises(ValueError, match="noise"):
+        gaussian_act(M, S, None)
+    with pytest.raises(ValueError, match="noise"):
+        gaussian_act(M, S, None, actions=f(5, 2))
+    with pytest.raises(ValueError, match="actions"):
+        gaussian_log_pi(M, S, None)
