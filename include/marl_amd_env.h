@@ -397,7 +397,8 @@ int asm_gated_scan_backward(int dtype, int64_t T, int64_t B, int64_t D, const vo
                             int64_t dx_st, int64_t dx_sb, float *dh0 /*nullable*/, const float *kept /*nullable*/, void *ws, int64_t ws_bytes,
                             void *stream);
 /* One step of a rollout: state [B][D] float32 is updated in place, out gets the new state in dtype.  Row b of gate, x and
- * out starts at b * *_sb; reset (nullable): element b at [b * r_sb], nonzero: the state counts as zero first. */
+ * out starts at b * *_sb; reset (nullable): element b at [b * r_sb], nonzero: the state counts as zero first.  state and out may each
+ * be gate or x itself (one address, one stride, one type); any other overlap is refused. */
 int asm_gated_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64_t gate_sb, const void *x, int64_t x_sb,
                         float *state, const uint8_t *reset /*nullable*/, int64_t r_sb, void *out, int64_t out_sb, void *stream);
 

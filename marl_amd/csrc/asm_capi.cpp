@@ -616,6 +616,54 @@ static int seq_ws(const char *fn, const void *ws, int64_t have, int64_t need)
     return 0;
 }
 
+// The bytes that a strided tensor lies in: w bytes at p + i s[0] + j s[1] + ..., strides positive (back: its own one was not) and in
+// descending order.
+struct Bytes {
+    intptr_t p;
+    int64_t w;
+    int nd;
+    int64_t n[3], s[3];
+    bool back[3];
+    Bytes(const void *ptr, int64_t elem) : p(reinterpret_cast<intptr_t>(ptr)), w(elem), nd(0) {}
+    void axis(int64_t count, int64_t stride)                            // (in bytes; one that is counted once, or an input's of 0, is none)
+    {
+        if (count <= 1 || stride == 0) return;
+        const bool b = stride < 0;
+        if (b) { p += (count - 1) * stride; stride = -stride; }
+        int k = nd++;
+        for (; k > 0 && s[k - 1] < stride; --k) { n[k] = n[k - 1]; s[k] = s[k - 1]; back[k] = back[k - 1]; }
+        n[k] = count; s[k] = stride; back[k] = b;
+    }
+    int64_t span() const { int64_t t = w; for (int k = 0; k < nd; ++k) t += (n[k] - 1) * s[k]; return t; }
+    Bytes inner() const { Bytes t = *this; t.nd = nd - 1; for (int k = 1; k < nd; ++k) { t.n[k - 1] = n[k]; t.s[k - 1] = s[k]; } return t; }
+};
+// Whether a and b, b's first byte `delta` behind a's, share a byte: the widest stride of the two is dealt with by its
+// multiples that bring the rest of both near enough, the rest by recursion.  More than 64 of those (rows that lie in each other): yes.
+static bool meet(int64_t delta, const Bytes &a, const Bytes &b)
+{
+    if (delta >= a.span() || -delta >= b.span()) return false;
+    if (!a.nd && !b.nd) return true;
+    const int64_t s = std::max(a.nd ? a.s[0] : 0, b.nd ? b.s[0] : 0);
+    const bool of_a = a.nd && a.s[0] == s, of_b = b.nd && b.s[0] == s;
+    const Bytes ra = of_a ? a.inner() : a, rb = of_b ? b.inner() : b;
+    // -span(rb) < delta + m s < span(ra), m = b's index - a's
+    const auto below = [](int64_t x, int64_t y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };       // (rounds down)
+    const int64_t lo = std::max(of_a ? 1 - a.n[0] : 0, below(-rb.span() - delta, s) + 1);
+    const int64_t hi = std::min(of_b ? b.n[0] - 1 : 0, -below(delta - ra.span(), s) - 1);
+    if (hi - lo >= 64) return true;
+    for (int64_t m = lo; m <= hi; ++m)
+        if (meet(delta + m * s, ra, rb)) return true;
+    return false;
+}
+static bool share(const Bytes &a, const Bytes &b) { return meet(b.p - a.p, a, b); }
+// One and the same layout: every thread reads the elements that it writes, before it writes them.
+static bool same(const Bytes &a, const Bytes &b)
+{
+    if (a.p != b.p || a.w != b.w || a.nd != b.nd) return false;
+    for (int k = 0; k < a.nd; ++k) if (a.n[k] != b.n[k] || a.s[k] != b.s[k] || a.back[k] != b.back[k]) return false;
+    return true;
+}
+
 int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
 {
     if (seq_dims("asm_gated_scan_workspace", dtype, T, B, D)) return -1;
@@ -674,6 +722,16 @@ int asm_gated_scan_step(int dtype, int64_t B, int64_t D, const void *gate, int64
     if (int rc = seq_dims("asm_gated_scan_step", dtype, 1, B, D)) return rc;
     if (B * D == 0) return 0;
     if (!gate || !x || !state || !out) return fail(1, "asm_gated_scan_step: NULL pointer");
+    const int64_t e = dtype ? 2 : 4;
+    const auto rows = [&](const void *p, int64_t sb, int64_t elem) { Bytes t(p, elem); t.axis(B, sb * elem); t.axis(D, elem); return t; };
+    const Bytes in[2] = {rows(gate, gate_sb, e), rows(x, x_sb, e)}, to[2] = {rows(state, D, 4), rows(out, out_sb, e)};
+    Bytes cut(reset, 1);
+    cut.axis(B, r_sb);
+    bool bad = share(to[0], to[1]);
+    for (const Bytes &o : to)
+        for (const Bytes &i : in) bad = bad || (!same(o, i) && share(o, i));
+    if (bad || (reset && (share(to[0], cut) || share(to[1], cut))))
+        return fail(1, "asm_gated_scan_step: state or out share memory with each other, with reset or, shifted, with gate or x");
     int rc = asmseq::launch_scan_step(dtype, B, D, gate, gate_sb, x, x_sb, state, reset, r_sb, out, out_sb, (hipStream_t)stream);
     return rc ? hip_fail(rc, "asm_gated_scan_step") : 0;
 }

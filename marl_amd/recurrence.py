@@ -180,8 +180,8 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
 def gated_scan_step(gate: torch.Tensor, x: torch.Tensor, state: torch.Tensor, *, reset: Optional[torch.Tensor] = None,
                     out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """One step of the memory in a rollout, without gradients: state (B, D) float32, contiguous, is updated in place, the
-    new state is returned in gate's type (in `out` if given; it may be gate or x itself, not the state).  reset: (B,) bool or uint8; where
-    set, the state counts as zero first."""
+    new state is returned in gate's type (in `out` if given; it may be gate or x itself, not the state, and may not overlap the
+    state, reset or, shifted, gate or x: refused).  reset: (B,) bool or uint8; where set, the state counts as zero first."""
     shape, dt, dev = gate.shape, gate.dtype, gate.device
     D = shape[-1] if shape else 0
     if out is None and dev.type == "cuda":
