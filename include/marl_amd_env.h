@@ -440,7 +440,8 @@ uint64_t asm_capture_id(void *stream);
 /* Multiplies n_mean values of dmean and n_std of dlog_std by *grad (device); reads and writes nothing when that is 1. */
 int asm_policy_loss_scale(int dtype, const float *grad, int64_t n_mean, void *dmean, int64_t n_std, void *dlog_std, void *stream);
 /* actions = mean + e^log_std noise (noise.p NULL: actions are given, not written) and log_pi of the actions as they are
- * stored in float32.  A log_std shared by all rows has sb = sn = 0. */
+ * stored in float32.  A log_std shared by all rows has sb = sn = 0.  actions, where written, may be mean, log_std or noise itself (one
+ * address, the same strides, float32); any other overlap of actions or log_pi, also of an output with itself, is refused. */
 int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_act_rows *rows, void *stream);
 
 /* Self-test hook: which kernel asm_batch_step_f32 would launch for these arguments: waves per workgroup of the

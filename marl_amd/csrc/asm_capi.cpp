@@ -616,23 +616,24 @@ static int seq_ws(const char *fn, const void *ws, int64_t have, int64_t need)
     return 0;
 }
 
-// The bytes that a strided tensor lies in: w bytes at p + i s[0] + j s[1] + ..., strides positive (back: its own one was not) and in
-// descending order.
+// The bytes that a strided tensor lies in: w bytes at p + i s[0] + j s[1] + ..., strides positive and in descending order; way: which
+// axis that is, negative where its own stride was.
 struct Bytes {
     intptr_t p;
     int64_t w;
     int nd;
     int64_t n[3], s[3];
-    bool back[3];
-    Bytes(const void *ptr, int64_t elem) : p(reinterpret_cast<intptr_t>(ptr)), w(elem), nd(0) {}
+    int way[3], axes;
+    Bytes(const void *ptr, int64_t elem) : p(reinterpret_cast<intptr_t>(ptr)), w(elem), nd(0), axes(0) {}
     void axis(int64_t count, int64_t stride)                            // (in bytes; one that is counted once, or an input's of 0, is none)
     {
+        ++axes;
         if (count <= 1 || stride == 0) return;
-        const bool b = stride < 0;
-        if (b) { p += (count - 1) * stride; stride = -stride; }
+        const int id = stride < 0 ? -axes : axes;
+        if (stride < 0) { p += (count - 1) * stride; stride = -stride; }
         int k = nd++;
-        for (; k > 0 && s[k - 1] < stride; --k) { n[k] = n[k - 1]; s[k] = s[k - 1]; back[k] = back[k - 1]; }
-        n[k] = count; s[k] = stride; back[k] = b;
+        for (; k > 0 && s[k - 1] < stride; --k) { n[k] = n[k - 1]; s[k] = s[k - 1]; way[k] = way[k - 1]; }
+        n[k] = count; s[k] = stride; way[k] = id;
     }
     int64_t span() const { int64_t t = w; for (int k = 0; k < nd; ++k) t += (n[k] - 1) * s[k]; return t; }
     Bytes inner() const { Bytes t = *this; t.nd = nd - 1; for (int k = 1; k < nd; ++k) { t.n[k - 1] = n[k]; t.s[k - 1] = s[k]; } return t; }
@@ -660,8 +661,27 @@ static bool share(const Bytes &a, const Bytes &b) { return meet(b.p - a.p, a, b)
 static bool same(const Bytes &a, const Bytes &b)
 {
     if (a.p != b.p || a.w != b.w || a.nd != b.nd) return false;
-    for (int k = 0; k < a.nd; ++k) if (a.n[k] != b.n[k] || a.s[k] != b.s[k] || a.back[k] != b.back[k]) return false;
+    for (int k = 0; k < a.nd; ++k) if (a.n[k] != b.n[k] || a.s[k] != b.s[k] || a.way[k] != b.way[k]) return false;
     return true;
+}
+
+// Whether two different elements of an output are one: along the widest axis first, then along the others.
+static bool folded(int64_t B, int64_t n, const asm_rows &r, int A, int64_t elem)
+{
+    const int64_t count[3] = {B, n, A}, stride[3] = {r.sb, r.sn, A > 1 ? r.sa : 0};
+    Bytes t(r.p, elem);
+    for (int k = 0; k < 3; ++k) {
+        if (count[k] > 1 && stride[k] == 0) return true;
+        t.axis(count[k], stride[k] * elem);
+    }
+    for (; t.nd; t = t.inner()) {
+        const Bytes rest = t.inner();
+        const int64_t near = std::min(t.n[0] - 1, (rest.span() - 1) / t.s[0]);
+        if (near >= 64) return true;
+        for (int64_t m = 1; m <= near; ++m)
+            if (meet(m * t.s[0], rest, rest)) return true;
+    }
+    return false;
 }
 
 int64_t asm_gated_scan_workspace(int dtype, int64_t T, int64_t B, int64_t D)
@@ -816,6 +836,19 @@ int asm_gaussian_act(int dtype, int64_t B, int64_t n, int A, const asm_act_rows 
     if (B * n == 0) return 0;
     if (!t || !t->mean.p || !t->log_std.p || !t->actions.p || !t->log_pi.p)
         return fail(1, "asm_gaussian_act: NULL pointer");
+    const int64_t e = dtype ? 2 : 4;
+    const auto bytes = [&](const asm_rows &r, int64_t elem, bool axis) {
+        Bytes b(r.p, elem);
+        b.axis(B, r.sb * elem); b.axis(n, r.sn * elem);
+        if (axis) b.axis(A, r.sa * elem);
+        return b;
+    };
+    const Bytes in[3] = {bytes(t->mean, e, true), bytes(t->log_std, e, true), bytes(t->noise, 4, true)};
+    const Bytes act = bytes(t->actions, 4, true), lp = bytes(t->log_pi, 4, false);
+    bool bad = share(act, lp) || folded(B, n, t->log_pi, 1, 4), own = t->noise.p != nullptr;        // (own: the actions are written)
+    bad = bad || (own && folded(B, n, t->actions, A, 4));
+    for (int k = 0; k < (own ? 3 : 2); ++k) bad = bad || share(lp, in[k]) || (own && !same(act, in[k]) && share(act, in[k]));
+    if (bad) return fail(1, "asm_gaussian_act: actions or log_pi lie in themselves, or share memory with each other or an input");
     asmseq::ActArgs a{};
     a.dtype = dtype; a.B = B; a.n = n; a.A = A;
     a.mean = rows_of(t->mean); a.log_std = rows_of(t->log_std); a.noise = rows_of(t->noise); a.actions = rows_of(t->actions); a.log_pi = rows_of(t->log_pi);

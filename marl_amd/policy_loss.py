@@ -194,7 +194,8 @@ def gaussian_act(mean: torch.Tensor, log_std: torch.Tensor, noise: torch.Tensor,
     """A rollout's actions, without gradients: (actions, log_pi) with actions = mean + e^log_std noise and log_pi the
     log-probability of the actions as they are stored in float32, so that a ratio taken from it later starts at 1.
     noise: standard normal draws of mean's shape (torch.randn); log_std: mean's shape, or (A,) for all rows.  actions, log_pi: where to write
-    (strided views are fine: DeviceReplay.action_slot().transpose(-1, -2))."""
+    (strided views are fine: DeviceReplay.action_slot().transpose(-1, -2); actions may be noise, mean or log_std itself; outputs that
+    overlap an input otherwise, each other or themselves are refused)."""
     _need(noise is not None, "gaussian_act: noise must be a float32 tensor of mean's shape")
     return _act("gaussian_act", mean, log_std, noise, actions, log_pi)
 

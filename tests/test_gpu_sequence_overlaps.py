@@ -24,3 +24,30 @@ def test_step(torch_cuda, B, D, dtype):
         with pytest.raises(RuntimeError, match="share memory"):
             gated_scan_step(gate, x, state, reset=r, out=out)
     assert torch.equal(buf, keep) and not bool(state.any())
+
+
+def test_actions(torch_cuda):
+    torch = torch_cuda
+    from marl_amd.policy_loss import gaussian_act, gaussian_log_pi
+    E, n, A = 5, 30, 2
+    buf = torch.randn(E, n, 4 * A + 1, device="cuda")
+    mean, std, noise, lp = buf[..., :A], buf[..., A:2 * A], buf[..., 2 * A:3 * A], buf[..., 4 * A]
+    want, wl = gaussian_act(mean.clone(), std.clone(), noise.clone())
+    for act in (buf[..., 3 * A:4 * A], noise, mean, std):               # a head's output and its actions in one buffer, then in place
+        b2 = buf.clone()
+        at = lambda t: b2.as_strided(t.shape, t.stride(), t.storage_offset())  # noqa: E731
+        got, gl = gaussian_act(at(mean), at(std), at(noise), actions=at(act), log_pi=at(lp))
+        assert torch.equal(got, want) and torch.equal(at(act), want) and torch.equal(gl, wl) and torch.equal(at(lp), wl)
+    ring = torch.zeros(3, E, A, n, device="cuda")                       # the replay's layout
+    gaussian_act(mean, std, noise, actions=ring[1].transpose(-1, -2), log_pi=ring[2, :, 0])
+    assert torch.equal(ring[1].transpose(-1, -2), want) and torch.equal(ring[2, :, 0], wl) and not bool(ring[0].any()) and not bool(ring[2, :, 1].any())
+    keep = buf.clone()
+    for kw in (dict(actions=buf[..., 1:A + 1]), dict(actions=buf[..., 2 * A + 1:3 * A + 1]), dict(log_pi=buf[..., 0]), dict(log_pi=buf[..., 3 * A - 1]),
+               dict(actions=buf[..., 3 * A:4 * A], log_pi=buf[..., 4 * A - 1])):
+        with pytest.raises(RuntimeError, match="share memory"):
+            gaussian_act(mean, std, noise, **kw)
+    with pytest.raises(RuntimeError, match="share memory"):
+        gaussian_log_pi(mean, std, noise, log_pi=buf[..., 2 * A])
+    with pytest.raises(RuntimeError, match="share memory"):             # rows of one output that lie in each other
+        gaussian_act(mean, std, noise, actions=torch.zeros(400, device="cuda").as_strided((E, n, A), (30, 1, 1)))
+    assert torch.equal(buf, keep)

@@ -70,3 +70,37 @@ def test_step_against_every_byte():
         assert _step(dtype, B, D, gate, x, state, reset, out) == bad, (dtype, B, D, gate, x, state, reset, out)
         seen[bad] += 1
     assert min(seen) > 100, seen
+
+
+def _act(dtype, B, n, A, mean, std, noise, actions, log_pi):
+    """Each: (address, strides of the three axes); noise: the same or None."""
+    import struct
+    lib = _lib.load()
+    rows = struct.pack("20q", *mean, *std, *(noise or (0, 0, 0, 0)), *actions, *log_pi)
+    assert lib.asm_gaussian_act(dtype, B, n, A, rows, None) != 0
+    return "share memory" in lib.asm_last_error().decode()
+
+
+def test_actions_against_every_byte():
+    rng = random.Random(11)
+    seen = [0, 0]
+    for _ in range(4000):
+        dtype, B, n, A = rng.randrange(2), rng.randrange(1, 4), rng.randrange(1, 4), rng.randrange(1, 4)
+        e = 2 if dtype else 4
+        full = lambda: rng.choice([(n * A, A, 1), (n * A, 1, n), (3 * n * A, 3 * A, 1), (3 * n * A, 1, 3 * n), (n * A + 2, A, 1), (1, B, B * n), (-n * A, A, 1)])  # noqa: E731
+        at = lambda elem: BASE + elem * rng.randrange(0, 70)  # noqa: E731
+        mean, std, noise, act = (at(e), *full()), (at(e), *rng.choice([full(), (0, 0, 1)])), rng.choice([None, (at(4), *full())]), (at(4), *full())
+        if noise and rng.random() < 0.3:
+            act = rng.choice([noise, mean])
+        lp = (at(4), *rng.choice([(n, 1), (3 * n, 3), (n + 1, 1), (1, B), (0, 1), (1, 1)]), 0)
+        axes = lambda t: ((B, t[1]), (n, t[2]), (A, t[3]))  # noqa: E731
+        M, S, U, L = _bytes(mean[0], e, *axes(mean)), _bytes(std[0], e, *axes(std)), _bytes(act[0], 4, *axes(act)), _bytes(lp[0], 4, (B, lp[1]), (n, lp[2]))
+        N = _bytes(noise[0], 4, *axes(noise)) if noise else []
+        bad = len(set(L)) < len(L) or bool(set(L) & (set(M) | set(S) | set(N) | set(U)))
+        if noise:
+            bad = bad or len(set(U)) < len(U)
+            for frm in (M, S, N):
+                bad = bad or (U != frm and bool(set(U) & set(frm)))
+        assert _act(dtype, B, n, A, mean, std, noise, act, lp) == bad, (dtype, B, n, A, mean, std, noise, act, lp)
+        seen[bad] += 1
+    assert min(seen) > 100, seen
