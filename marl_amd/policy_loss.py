@@ -15,7 +15,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from .recurrence import _DTYPES, _FLAGS, _call, _capture, _guard_leaves, _need, _on_device, _once, _ptr, _workspace
+from .recurrence import _DTYPES, _FLAGS, _call, _capture, _guard_leaves, _need, _no_tangents, _on_device, _once, _ptr, _workspace
 
 STATS_FIELDS = ("gain", "kl", "entropy", "clipped", "ratio", "rows")
 _NO_ROWS = (0, 0, 0, 0)
@@ -170,6 +170,7 @@ def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torc
                                               (log_pi_ref is not None and log_pi_ref.requires_grad) or
                                               (adv_moments is not None and adv_moments.requires_grad)))):
         _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv_moments, clip, kl_coef, entropy_coef)
+    _no_tangents("clipped_policy_loss", mean, log_std, actions, log_pi_old, adv, log_pi_ref, adv_moments)
     shared = int(log_std.shape == mean.shape[-1:])
     adv_moments = None if adv_moments is None else adv_moments.contiguous()
     loss, stats = _ClippedLoss.apply(mean, log_std, (actions, log_pi_old, log_pi_ref, adv, mask, adv_moments),

@@ -13,6 +13,7 @@ from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -64,6 +65,14 @@ def _call(name: str, dev: torch.device, *args) -> None:
             rc = fn(*args, _raw_stream(index))
     if rc:
         _lib.check(rc, name)
+
+
+def _no_tangents(fn: str, *tensors) -> None:
+    """(an operator that is not entered through its autograd function would drop a dual tensor's tangent without a word)"""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{fn} has no forward-mode derivative: its inputs may not be dual tensors")
 
 
 def _once(fn: str) -> None:
@@ -168,6 +177,7 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
             (resets is None or (resets.shape == shape[:2] and resets.dtype in _FLAGS and resets.device == dev)) and
             (lengths is None or (lengths.shape == (B,) and lengths.dtype == torch.int32 and lengths.device == dev))):
         _explain_scan(gate, x, h0, resets, lengths, B, D)
+    _no_tangents("gated_scan", gate, x, h0)
     gate, x = _dense(gate), _dense(x)
     h0 = None if h0 is None else h0.contiguous()
     lengths = None if lengths is None else lengths.contiguous()
