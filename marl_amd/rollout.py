@@ -90,6 +90,28 @@ class _FlatGrads:
         self.flat.div_(dist.get_world_size(group))
 
 
+def _several_ranks(group=None) -> bool:
+    return dist.is_available() and dist.is_initialized() and dist.get_world_size(group) > 1
+
+
+def _replicated(data_parallel: bool, group) -> bool:
+    """Whether a learner is one of several replicas."""
+    if data_parallel and not (dist.is_available() and dist.is_initialized()):
+        raise RuntimeError("data_parallel=True needs torch.distributed.init_process_group() first")
+    return bool(data_parallel) and _several_ranks(group)
+
+
+def _take_weights_of_rank_0(nets, group) -> None:
+    for net in nets:                                                       # one message per network
+        flat = torch.cat([p.data.reshape(-1) for p in net.parameters()])
+        if dist.get_rank(group) != 0:                                      # SUM of (rank 0's weights, zeros, ...) = a broadcast
+            flat.zero_()
+        all_reduce_sum(flat, group)
+        off = 0
+        for p in net.parameters():
+            p.data.copy_(flat[off:off + p.numel()].view_as(p)); off += p.numel()
+
+
 def _obs_rows(obs: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
     """(E, obs_dim, n_a) float32 frames on the device -> rows (E * n_a, obs_dim), one per agent (asm_obs_rows_f32)."""
     from . import _lib
@@ -116,19 +138,9 @@ class DDPGLearner:
         self.policy, self.target_policy = mk(obs_dim, act_dim, True), mk(obs_dim, act_dim, True)
         self.critic, self.target_critic = mk(obs_dim + act_dim, 1, False), mk(obs_dim + act_dim, 1, False)
         self.group = group
-        self.data_parallel = bool(data_parallel) and dist.is_available() and dist.is_initialized() and \
-            dist.get_world_size(group) > 1
-        if data_parallel and not (dist.is_available() and dist.is_initialized()):
-            raise RuntimeError("data_parallel=True needs torch.distributed.init_process_group() first")
+        self.data_parallel = _replicated(data_parallel, group)
         if self.data_parallel:
-            for net in (self.policy, self.critic):                         # one message per network
-                flat = torch.cat([p.data.reshape(-1) for p in net.parameters()])
-                if dist.get_rank(group) != 0:                              # SUM of (rank 0's weights, zeros, ...) = a broadcast
-                    flat.zero_()
-                all_reduce_sum(flat, group)
-                off = 0
-                for p in net.parameters():
-                    p.data.copy_(flat[off:off + p.numel()].view_as(p)); off += p.numel()
+            _take_weights_of_rank_0((self.policy, self.critic), group)
         self.target_policy.load_state_dict(self.policy.state_dict())       # agents.py:39-40
         self.target_critic.load_state_dict(self.critic.state_dict())
         self.policy_optimizer = torch.optim.Adam(self.policy.parameters(), lr_actor, capturable=capturable)
@@ -283,15 +295,24 @@ class ClippedPolicyLearner:
     on whole episodes with the clipped policy loss, and a critic of the state alone whose values give the advantages.
 
     run_episode() with a DeviceReplay(..., log_pi=True) records an episode under it, train_on_policy() updates it from that
-    episode.  Memories are kept for each group of environments (by its first global id) and cleared by begin_episode()."""
+    episode.  Memories are kept for each group of environments (by its first global id) and cleared by begin_episode().
+
+    data_parallel=True, group: replicas on several ranks as DDPGLearner's: rank 0's initial weights for all, one SUM all-reduce
+    of a network's flattened gradient divided by the number of ranks in front of each optimiser step, and advantages normalised
+    over all ranks' episodes.  Without it, update() refuses a process group of several ranks, whose replicas would drift apart."""
 
     def __init__(self, obs_dim: int, act_dim: int = 2, hidden_dim: int = 256, lr_actor: float = 3e-4, lr_critic: float = 1e-3,
                  gamma: float = 0.95, lam: float = 0.95, clip: float = 0.2, kl_coef: float = 0.0, entropy_coef: float = 0.0,
-                 init_std: float = 0.5, device="cuda"):
+                 init_std: float = 0.5, device="cuda", data_parallel: bool = False, group=None):
         self.policy = MemoryPolicy(obs_dim, act_dim, hidden_dim, init_std).to(device)
         self.critic = MLPNetwork(obs_dim, 1, hidden_dim).to(device)
+        self.group, self.data_parallel = group, _replicated(data_parallel, group)
+        if self.data_parallel:
+            _take_weights_of_rank_0((self.policy, self.critic), group)
         self.policy_optimizer = torch.optim.Adam(self.policy.parameters(), lr_actor)
         self.critic_optimizer = torch.optim.Adam(self.critic.parameters(), lr_critic)
+        self._pol_grads = _FlatGrads(self.policy) if self.data_parallel else None
+        self._cri_grads = _FlatGrads(self.critic) if self.data_parallel else None
         self.gamma, self.lam, self.clip, self.kl_coef, self.entropy_coef = gamma, lam, clip, kl_coef, entropy_coef
         self.fused_policy, self._explore_step = None, 0                    # (read by the loops written for DDPGLearner)
         self._row_bufs = {}
@@ -331,26 +352,49 @@ class ClippedPolicyLearner:
 
     def update(self, frames, actions, log_pi, adv, ret, moments):
         """One step of both optimisers on an episode of some environments: frames (T, E, obs_dim, n_a), actions (T, E, act_dim, n_a),
-        log_pi, adv and ret (T, E, n_a).  Returns (policy loss, critic loss, stats) as tensors (policy_loss.STATS_FIELDS)."""
+        log_pi, adv and ret (T, E, n_a).  Returns (policy loss, critic loss, stats) as tensors (policy_loss.STATS_FIELDS), of this
+        rank's rows.  data_parallel: every rank makes the same calls with as many rows."""
+        if not self.data_parallel and _several_ranks(self.group):
+            raise RuntimeError("several ranks, each with episodes of its own: ClippedPolicyLearner(..., data_parallel=True), or a group of this rank alone")
         T, E, _, n = frames.shape
         rows = self._rows(frames)
         mean, _ = self.policy(rows)
         loss, stats = clipped_policy_loss(mean.view(T, E, n, -1), self.policy.log_std, actions.transpose(2, 3), log_pi, adv, adv_moments=moments,
                                           clip=self.clip, kl_coef=self.kl_coef, entropy_coef=self.entropy_coef)
-        self.policy_optimizer.zero_grad()
-        loss.backward()
-        self.policy_optimizer.step()
+        self._step(loss, self.policy_optimizer, self._pol_grads)
         vf_loss = F.mse_loss(self.critic(rows).view(T, E, n), ret)
-        self.critic_optimizer.zero_grad()
-        vf_loss.backward()
-        self.critic_optimizer.step()
+        self._step(vf_loss, self.critic_optimizer, self._cri_grads)
         return loss.detach(), vf_loss.detach(), stats
+
+    def _step(self, loss, optimizer, flat) -> None:
+        if flat is None:
+            optimizer.zero_grad()
+        else:
+            flat.zero()
+        loss.backward()
+        if flat is not None:
+            flat.average(self.group)
+        optimizer.step()
+
+
+def _over_ranks(moments: torch.Tensor, sizes, group) -> torch.Tensor:
+    """The moments of all ranks' advantages from each rank's own, and a check that all ranks train on as much, in one message: ranks
+    with other numbers of updates would wait for each other for good."""
+    mean, sd = moments[0].double(), 1.0 / moments[1].double() - 1e-8
+    own = torch.tensor([float(s) for s in sizes], dtype=torch.float64, device=moments.device)
+    v = all_reduce_sum(torch.cat((own, own * own, torch.stack((mean, mean * mean + sd * sd)))), group)
+    world, host, k = dist.get_world_size(group), v.tolist(), len(sizes)
+    if any(world * sq != s * s for s, sq in zip(host[:k], host[k:2 * k])):      # (equal exactly where all ranks' numbers are)
+        raise RuntimeError("train_on_policy: the ranks differ in episode length, environments, agents, epochs or envs_per_batch")
+    mean, square = v[-2] / world, v[-1] / world
+    return torch.stack((mean, 1.0 / ((square - mean * mean).clamp_min(0.0).sqrt() + 1e-8))).float()
 
 
 def train_on_policy(env: BatchedAssemblyEnv, learner: ClippedPolicyLearner, replay: DeviceReplay, epochs: int = 4, envs_per_batch: int = 64):
     """The on-policy counterpart of train_phase(): `epochs` passes over the episode run_episode() left in the replay's current
     slot, envs_per_batch environments at a time, in order.  Returns a (updates, 8) tensor: policy loss, critic loss and
-    policy_loss.STATS_FIELDS of each update; nothing is read back in between."""
+    policy_loss.STATS_FIELDS of each update, of this rank's rows; nothing is read back in between (a data-parallel learner reads
+    a few numbers once, to see that its ranks train alike)."""
     k = replay.slot
     if k < 0 or not replay.complete[k] or replay.log_pi_ring is None:
         raise RuntimeError("train_on_policy needs a complete episode recorded with DeviceReplay(..., log_pi=True)")
@@ -362,6 +406,8 @@ def train_on_policy(env: BatchedAssemblyEnv, learner: ClippedPolicyLearner, repl
         for g in groups:
             values[:, g] = learner.critic(learner._rows(frames[:, g])).view(T + 1, -1, env.n_a)
     adv, ret, moments = replay.advantages(values, gamma=learner.gamma, lam=learner.lam)
+    if learner.data_parallel:
+        moments = _over_ranks(moments, (T, E, env.n_a, epochs, envs_per_batch), learner.group)
     out = []
     for _ in range(epochs):
         for g in groups:
