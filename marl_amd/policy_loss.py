@@ -135,6 +135,7 @@ def _loss(mean, log_std, actions, old, ref, adv, mask, moments, shared, clip, kl
     dstd = torch.empty(log_std.shape, dtype=dt, device=dev)
     need = _loss_workspace(B * n, A)
     ws = _workspace(need, dev)
+    moments = None if moments is None else moments.contiguous()
     r0, k0 = _rows(mean, lead, True)                                    # (k: the tensors a copy may have been made of)
     r1, k1 = _rows_std(log_std, lead, shared)
     r2, k2 = _rows(actions, lead, True)
@@ -172,7 +173,6 @@ def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torc
         _explain_loss(mean, log_std, actions, log_pi_old, adv, log_pi_ref, mask, adv_moments, clip, kl_coef, entropy_coef)
     _no_tangents("clipped_policy_loss", mean, log_std, actions, log_pi_old, adv, log_pi_ref, adv_moments)
     shared = int(log_std.shape == mean.shape[-1:])
-    adv_moments = None if adv_moments is None else adv_moments.contiguous()
     loss, stats = _ClippedLoss.apply(mean, log_std, (actions, log_pi_old, log_pi_ref, adv, mask, adv_moments),
                                      (shared, float(clip), float(kl_coef), float(entropy_coef)))
     return (_guard_leaves(loss, mean.device) if loss.requires_grad else loss), stats

@@ -146,6 +146,7 @@ class _GatedScan(torch.autograd.Function):
         _once("gated_scan")
         gate, x, h, h0, resets, lengths, kept = ctx.saved_tensors
         gate, x, h = _dense(gate), _dense(x), _dense(h)                  # (saved-tensor hooks may hand back other strides)
+        h0, lengths, kept = (None if t is None else t.contiguous() for t in (h0, lengths, kept))
         T, B, D = ctx.dims
         bf, dev, dt = ctx.batch_first, gate.device, _DTYPES[gate.dtype]
         dh = None if dh is None else _dense(dh)

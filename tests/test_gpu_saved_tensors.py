@@ -41,3 +41,37 @@ def test_saved_tensors_may_come_back_transposed(torch_cuda):
     got = torch.autograd.grad((h, last), leaves, (dh, dl))
     want = torch.autograd.grad(gated_scan(*leaves), leaves, (dh, dl))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_every_saved_tensor_may_come_back_strided(torch_cuda, dtype):
+    """States, lengths, resets and advantage moments too; the loss reads its saved tensors in a second backward pass."""
+    torch = torch_cuda
+    from marl_amd.policy_loss import clipped_policy_loss
+    from marl_amd.recurrence import gated_scan
+    T, B, D = 9, 4, 6
+
+    def spread(t):                                                      # twice as far apart along every axis, something else between
+        wide = torch.full([2 * n for n in t.shape], 7, device=t.device).to(t.dtype)
+        out = wide[tuple(slice(0, None, 2) for _ in t.shape)]
+        out.copy_(t)
+        return out
+
+    dt = getattr(torch, dtype)
+    leaves = [torch.randn(T, B, D, device="cuda").to(dt).requires_grad_(), torch.randn(T, B, D, device="cuda").to(dt).requires_grad_(),
+              torch.randn(B, D, device="cuda", requires_grad=True)]
+    kw = dict(resets=torch.rand(T, B, device="cuda") < 0.2, lengths=torch.tensor([9, 0, 4, 7], device="cuda", dtype=torch.int32))
+    dh, dl = torch.randn(T, B, D, device="cuda").to(dt), torch.randn(B, D, device="cuda")
+    want = torch.autograd.grad(gated_scan(*leaves, **kw), leaves, (dh, dl))
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        out = gated_scan(*leaves, **kw)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(out, leaves, (dh, dl)), want))
+    rows = [torch.randn(50, 2, device="cuda", requires_grad=True), torch.zeros(2, device="cuda", requires_grad=True), torch.randn(50, 2, device="cuda"),
+            torch.randn(50, device="cuda"), torch.randn(50, device="cuda")]
+    kw = dict(adv_moments=torch.tensor([0.3, 1.7], device="cuda"), mask=torch.rand(50, device="cuda") < 0.7, kl_coef=0.1)
+    want = torch.autograd.grad(clipped_policy_loss(*rows, **kw)[0], rows[:2])
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, spread):
+        loss, _ = clipped_policy_loss(*rows, **kw)
+    for _ in range(2):
+        got = torch.autograd.grad(loss, rows[:2], retain_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
