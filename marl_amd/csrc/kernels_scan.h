@@ -430,6 +430,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
     const int lo = split * q.Ts, hi = lo + q.Ts < q.T ? lo + q.Ts : q.T;
     typename Op::Raw raw[L];
     float state[V];                                                     // BLOCK: the state in front of this wave's steps
+    static_assert(!AGG || NW > 1, "a wave that has all of time to itself composes nothing");
     static_assert(!Op::BLOCK || L == 8, "states are kept in front of every eighth step");
     auto step_at = [&](int u0, int l) __attribute__((always_inline)) { return Op::REVERSE ? Step{q.T - 1 - u0, -l} : Step{u0, l}; };
     // CLAMP: a step beyond the end reads the last one again, and is not used
@@ -499,7 +500,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
 #pragma unroll
         for (int l = 0; l < L; ++l) {
             op.coef(it[l], raw[l], ln, step_at(u0, l), FULL || u0 + l < hi);
-            if (NW > 1 || AGG) {
+            if (NW > 1) {
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
                     const bool cut = CUTS && cut_of(it[l], v);
@@ -528,13 +529,6 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
                 }
             }
             par ^= 1;                                                   // (the next tile's pairs go to the other half: one barrier a tile)
-        } else if (AGG) {
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float A = CUTS && any[v] ? -0.f : PA[v];
-                c[v] = through<CUTS>(A, PS[v], c[v]);
-                CA[v] = joined<CUTS>(A, CA[v]);
-            }
         }
         if (!AGG) {
             const int kept = (q.T - u0) & 7;                            // the step of these, if any, in front of which the state is kept
