@@ -83,9 +83,10 @@ def _once(fn: str) -> None:
 
 def _capture(dev: torch.device) -> int:
     """The capture into a HIP graph that dev's current stream is part of, 0 for none."""
-    if torch.cuda.current_device() == dev.index and not torch.cuda.is_current_stream_capturing():
-        return 0
-    return _lib.load().asm_capture_id(_raw_stream(dev.index))
+    if torch.cuda.current_device() != dev.index:
+        with torch.cuda.device(dev):
+            return _capture(dev)
+    return _lib.load().asm_capture_id(_raw_stream(dev.index)) if torch.cuda.is_current_stream_capturing() else 0
 
 
 def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
@@ -96,7 +97,7 @@ def _guard_leaves(out: torch.Tensor, device) -> torch.Tensor:
     for node, _ in out.grad_fn.next_functions:
         if type(node).__name__ == "AccumulateGrad":
             first = node.metadata.setdefault("marl_amd_stream", stream)
-            if first != stream and torch.cuda.is_current_stream_capturing():
+            if first != stream and _capture(device):
                 raise RuntimeError("captured into a HIP graph while an autograd graph of the same leaf tensor, made on another stream, is alive: "
                                    "drop it (its loss and outputs) before capturing")
     return out

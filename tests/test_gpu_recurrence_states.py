@@ -49,3 +49,47 @@ def test_the_gates_gradient_of_strided_tensors(torch_cuda):
         for a, b, what in ((both[..., :D], both[..., D:2 * D], "aligned cut"), (both[..., 1:D + 1], both[..., D + 2:2 * D + 2], "odd offset"),
                            (both[..., 2:D + 2], both[..., D + 2:2 * D + 2], "two values aligned")):
             _check(torch, a, b, None, None, None, False, what)
+
+
+def _through_c(torch, gate, x, r, dh, flip, keep):
+    """Forward and backward pass through the C entries, time-major; flip: every tensor is walked backwards along that axis."""
+    from marl_amd import _lib
+    lib, dt = _lib.load(), _lib.SEQ_BF16
+    T, B, D = gate.shape
+    h, dgate, dx = (torch.zeros_like(gate) for _ in range(3))
+
+    def at(t):
+        s = list(t.stride()[:2])
+        p = t.data_ptr()
+        if flip is not None:
+            p += (t.shape[flip] - 1) * s[flip] * t.element_size()
+            s[flip] = -s[flip]
+        return (p, *s)
+    st = torch.cuda.current_stream().cuda_stream
+    need, size = lib.asm_gated_scan_workspace(dt, T, B, D), lib.asm_gated_scan_kept(dt, T, B, D)
+    assert size == (T + 7) // 8 * B * D * 4
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    kept = torch.full((size // 4,), float("nan"), device="cuda") if keep else None
+    pk = kept.data_ptr() if keep else None
+    _lib.check(lib.asm_gated_scan_forward(dt, T, B, D, *at(gate), *at(x), None, *at(r), None, *at(h), None, pk, ws.data_ptr(), need, st), "forward")
+    _lib.check(lib.asm_gated_scan_backward(dt, T, B, D, *at(gate), *at(x), *at(h), None, *at(r), None, *at(dh), None, *at(dgate), *at(dx), None, pk, ws.data_ptr(), need,
+                                           st), "backward")
+    return h, dgate, dx
+
+
+@pytest.mark.parametrize("flip", [None, 0, 1])
+@pytest.mark.parametrize("T,B,D", [(19, 500, 64), (19, 500, 256), (19, 1000, 256), (13, 7, 9), (350, 3, 30)])
+def test_c_entries_with_and_without_kept_states(torch_cuda, T, B, D, flip):
+    torch = torch_cuda
+    g = torch.Generator(device="cuda").manual_seed(T + D)
+    gate, x, dh = (torch.randn(T, B, D, device="cuda", generator=g).to(torch.bfloat16) for _ in range(3))
+    r = (torch.rand(T, B, device="cuda", generator=g) < 0.1).to(torch.uint8)
+    turned = lambda t: t if flip is None else t.flip(flip)  # noqa: E731
+    for keep in (True, False):
+        got = [turned(t) for t in _through_c(torch, gate, x, r, dh, flip, keep)]
+        if keep:
+            want = _want(turned(gate), turned(x), None, turned(r) != 0, None, False, turned(dh), torch.zeros(B, D))
+        else:                                                           # (the states are h as stored: seq_oracle's own bound)
+            want = so.scan(turned(gate), turned(x), resets=turned(r) != 0, dh=turned(dh))
+        for name, t in zip(("h", "dgate", "dx"), got):
+            so.within(t, *want[name], f"flip {flip} kept {keep} {name}")
