@@ -32,8 +32,8 @@
 //
 // What bounds the phases of a workgroup (cycle stamps, hidden width 256, 192 features, 30 agents): layer 1 and the
 // prologue by the observation stream (every workgroup of the chip is in that phase at the same time); the hidden
-// layers by the matrix core plus the issue cost of the weight copies; the activations by their ~900 vector
-// instructions (256 accumulator reads, bias adds and 0.01 products, 256 max, 128 packs).
+// layers by the matrix core plus the issue cost of the weight copies; the activations by their 1152 vector
+// instructions (256 accumulator reads, 256 bias adds, 256 0.01 products, 256 max, 128 packs).  4096 x 30 agents: 65 us.
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));

@@ -19,9 +19,9 @@
 // the chip, the time axis is cut into `nsplit` stretches: a first launch composes each stretch (its reads leave the data
 // in the last-level cache for the second), the second one starts each stretch from the composition of those before it.
 //
-// Measured: 200 steps x 491520 channels of float32 forward 235 us for 1.23 GB (5.2 TB/s, what a copy reaches: bound by HBM), 200 x 62848
-// of bfloat16 with resets and lengths 21 us for 76 MB (3.7 TB/s: 26 vector instructions an element and a step), 37 x 1920 3.8 us
-// (a launch and two trips to memory).
+// Measured: 200 steps x 491520 channels of float32 forward 241 us for 1.23 GB (5.1 TB/s, what a copy reaches: bound by HBM), 200 x 62848
+// of bfloat16 with resets and lengths forward 25 us for 83 MB (3.3 TB/s: 31 vector instructions an element and a step), backward 40 us
+// for 133 MB (72 of them, 25 us of issue; two waves a SIMD cover the rest badly), 37 x 1920 3.9 us (a launch and two trips to memory).
 //
 // Addresses: a tensor's base at this step and at the workgroup's first sequence is uniform (scalar registers), a lane adds a
 // 32-bit byte offset (OFF = uint32_t), or a 64-bit one where a workgroup's sequences lie too far apart (OFF = int64_t).
@@ -316,7 +316,7 @@ template <typename T, int V, bool MSK, typename OFF, bool KEPT> struct BackwardA
 template <typename T, int V, bool MSK, typename OFF> using BackwardOp = BackwardAnyOp<T, V, MSK, OFF, false>;
 template <typename T, int V, bool MSK, typename OFF> using BackwardKeptOp = BackwardAnyOp<T, V, MSK, OFF, true>;
 
-// 200 x 122880: 76 us for 395 MB (5.2 TB/s, bound by HBM).
+// 200 x 122880: 78 us for 395 MB (5.1 TB/s, bound by HBM).
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.
 template <int V, bool MSK, bool MOM> struct AdvantageOp {
     static constexpr bool REVERSE = true, SUMS = true, MOMENTS = MOM, CUTS = MSK, KEEPS = false, BLOCK = false;
@@ -580,7 +580,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
 }
 
 // The backward pass of many channels, one wave for all of time, from the states that the forward pass kept: it reads gate, x, dh
-// and an eighth of a state instead of gate, x, dh and h (200 x 1920 x 256 float32: 384 us for 2.0 GB, 460 us with h).
+// and an eighth of a state instead of gate, x, dh and h (200 x 1920 x 256 float32: 386 us for 2.0 GB, 460 us with h).
 template <typename T, int V, bool MSK>
 __global__ __launch_bounds__(64) void k_scan_back_kept(BackwardKeptOp<T, V, MSK, uint32_t> op, ScanGeom q)
 {
@@ -683,7 +683,7 @@ __global__ __launch_bounds__(256) void k_moments(const double *mom, int64_t n, f
     }
 }
 
-// (122880 x 256 float32: 115 us for 630 MB, bound by HBM; 30 x 64: 2.0 us, a launch.)
+// (122880 x 256 float32: 113 us for 630 MB, bound by HBM; 30 x 64: 2.2 us, a launch.)
 // One step of the memory: state <- a k state + (1 - a) x, out = the new state in the inputs' type.
 template <typename T, int V>
 __global__ __launch_bounds__(256) void k_scan_step(uint32_t n, uint32_t D, const void *gate, int64_t g_sb, const void *x, int64_t x_sb,

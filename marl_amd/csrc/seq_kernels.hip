@@ -32,20 +32,20 @@ struct Plan { int V, NW, L, nsplit, Ts; };
 
 // By C, the channels, and `size`, the bytes of a value (forward + backward of 200 steps, float32 / bfloat16, us):
 //   C       1 channel a lane, 4 waves a tile   2 channels, 4 waves   4 channels, one wave walks all of time
-//   30720              39 / 32                      41 / 32                     110 / 114
-//   62848              77 / 49                      75 / 42                     105 / 96
-//   122880            179 / 97                     162 / 79                     157 / 109
-//   245760            361 / 205                    357 / 174                    292 / 161
-//   491520            706 / 401                    691 / 358                    613 / 315
+//   30720              40 / 35                      42 / 34                     123 / 121
+//   62848              77 / 49                      76 / 46                     135 / 122
+//   122880            177 / 96                     166 / 85                     165 / 137
+//   245760            360 / 196                    357 / 177                    300 / 166
+//   491520            704 / 381                    691 / 346                    619 / 324
 // Many channels fill the chip by themselves, a wave that shares nothing waits for nobody, and its backward pass needs not read
-// h (k_scan_back_kept): from 480 KB a time step on.  Below, four waves side by side in time; from 49152 channels on two of
-// them in a lane (half the address work).  Rows that are not aligned to two or four
-// values go one channel a lane.
+// h, in float32 either (k_scan_back_kept): from 480 KB a time step on.  Below, four waves side by side in time; from 49152 channels on two of
+// them in a lane (half the address work; a backward pass from kept states eight steps a wave and tile).  Rows that are not aligned to
+// two or four values go one channel a lane.
 // Fewer than 256 workgroups of one channel a lane: what counts is how often a tile's loads are waited for.  Up to `whole` steps eight
 // waves share a tile and one launch does it all; from there on the time axis is cut until there are 512 workgroups, down to one tile
-// a stretch (1920 channels, forward + backward, us: 100 steps eight waves 13, four 14, cut 15; 200 steps 19, 22, 16; 333 steps
-// 24, 31, 19; 2000 steps 95, 144, 39; on the host each of the two launches more costs 4 us or, in a backward pass, up to 20.
-// 20011 steps x 183 channels: 61 stretches 97 us, 157 stretches 58 us).
+// a stretch (1920 channels, forward + backward, us: 100 steps eight waves 14, four 15, cut 15; 200 steps 20, 24, 16; 333 steps
+// 27, 34, 19; 2000 steps 111, 166, 42; on the host each of the two launches more costs 4 us or, in a backward pass, up to 20.
+// 20011 steps x 183 channels: 61 stretches 97 us, 157 stretches 53 us).
 Plan scan_plan(int64_t T, int64_t C, size_t size, bool vec2, bool vec4, int64_t whole = 320)
 {
     Plan p{1, 4, 8, 1, 0};

@@ -161,7 +161,11 @@ def clipped_policy_loss(mean: torch.Tensor, log_std: torch.Tensor, actions: torc
     none.  What a masked row holds does not matter.  Differentiable (once) in mean and log_std; the gradients are computed in
     the same pass.  log_std: mean's shape, or (A,) for all rows.  adv_moments: the (mean, 1 / deviation) that
     advantages(..., moments=True) returns; A = (adv - mean) / deviation then, else A = adv.
-    stats: 6 floats, STATS_FIELDS (means over the valid rows of min(..), e^D - 1 - D, H, rows cut off, q; the rows)."""
+    stats: 6 floats, STATS_FIELDS (means over the valid rows of min(..), e^D - 1 - D, H, rows cut off, q; the rows).  The mean of
+    e^D - 1 - D estimates KL(pi || pi_ref) without bias for actions drawn from pi itself: near the first update after the rollout.
+    For actions of an older policy, and with that policy as the reference, it is a distance (0 where the two agree) but no such estimate.
+    A row is computed in double and rounded once; with kl_coef = 0 that term takes no part, however far off a row is.
+    Without gradients enabled they are computed all the same."""
     dev, lead = mean.device, mean.shape[:-1]
     if not (_policy_ok(mean, log_std, (actions,), (log_pi_old, log_pi_ref, adv)) and
             (mask is None or (mask.shape == lead and mask.dtype in _FLAGS and mask.device == dev)) and

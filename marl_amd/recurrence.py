@@ -171,7 +171,8 @@ def gated_scan(gate: torch.Tensor, x: torch.Tensor, h0: Optional[torch.Tensor] =
     front of the first step (None: zeros).  resets: bool or uint8 of gate's first two axes; where set, the state counts as
     zero in front of that step, whatever it holds, and no gradient passes.  lengths: (B,) int32, clamped to 0..T: steps from
     there on are no part of the sequence; h and the gradients are zero there, and what gate and x hold does not matter.
-    Sequences may be of length 0."""
+    Sequences may be of length 0.  The backward pass works from float32 states: those in front of every eighth step are kept for it
+    (T B D / 2 bytes; float32 with less than 480 KB a step takes them from h)."""
     shape, dev = gate.shape, gate.device
     T, B, D = shape if len(shape) == 3 and not batch_first else (shape[1], shape[0], shape[2]) if len(shape) == 3 else (0, 0, 0)
     if not (len(shape) == 3 and x.shape == shape and gate.dtype in _DTYPES and x.dtype == gate.dtype and dev.type == "cuda" and x.device == dev and

@@ -82,3 +82,28 @@ def test_an_eager_backward_pass_of_a_captured_loss_keeps_its_gradients(torch_cud
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("T,B,D", [(600, 3, 20), (20, 7, 64), (20, 1200, 256)])
+def test_the_memorys_backward_pass_captured_alone(torch_cuda, no_garbage, T, B, D, dtype):
+    torch = torch_cuda
+    from marl_amd.recurrence import gated_scan
+    L = [torch.randn(T, B, D, device="cuda").to(getattr(torch, dtype)).requires_grad_() for _ in range(2)]
+    dh = torch.randn(T, B, D, device="cuda").to(getattr(torch, dtype))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        h, last = gated_scan(*L)
+        want = [t.clone() for t in torch.autograd.grad(h, L, dh, retain_graph=True)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(h, L, dh)
+    for k in range(3):
+        for t in got:
+            t.fill_(7.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
