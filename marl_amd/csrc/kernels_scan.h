@@ -316,6 +316,42 @@ template <typename T, int V, bool MSK, typename OFF, bool KEPT> struct BackwardA
 template <typename T, int V, bool MSK, typename OFF> using BackwardOp = BackwardAnyOp<T, V, MSK, OFF, false>;
 template <typename T, int V, bool MSK, typename OFF> using BackwardKeptOp = BackwardAnyOp<T, V, MSK, OFF, true>;
 
+// Number, mean and sum of squared distances from the mean of some values, in double.  add(): distances from the first of them;
+// join(): two sets' means differ by d, which adds d^2 n1 n2 / (n1 + n2) (Chan, Golub and LeVeque).  (A mean of squares less the square of
+// the mean would leave a deviation of 1e-8 of the mean where all values are equal.)
+struct Spread { double n, mean, m2; };
+struct SpreadSum {
+    double first = 0.0, s = 0.0, ss = 0.0;
+    int n = 0;
+    __device__ __forceinline__ void add(double x)
+    {
+        first = n ? first : x;
+        const double d = x - first;
+        s += d; ss = __fma_rn(d, d, ss); ++n;
+    }
+    __device__ Spread spread() const
+    {
+        if (!n) return {0.0, 0.0, 0.0};
+        const double m = s / n;
+        return {(double)n, first + m, ss - s * m > 0.0 || ss != ss ? ss - s * m : 0.0};
+    }
+};
+__device__ __forceinline__ Spread join(const Spread &a, const Spread &b)
+{
+    const double n = a.n + b.n, d = b.mean - a.mean, w = n > 0.0 ? b.n / n : 0.0;
+    if (a.n == 0.0) return b;
+    return b.n == 0.0 ? a : Spread{n, a.mean + d * w, a.m2 + b.m2 + d * d * a.n * w};
+}
+__device__ __forceinline__ Spread wave_join(Spread x)
+{
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const Spread y{__shfl_xor(x.n, o, 64), __shfl_xor(x.mean, o, 64), __shfl_xor(x.m2, o, 64)};
+        x = threadIdx.x & o ? join(y, x) : join(x, y);
+    }
+    return x;
+}
+
 // 200 x 122880: 78 us for 395 MB (5.1 TB/s, bound by HBM).
 // MSK: lengths or dones given.  Rows of one time step are contiguous (C channels), lengths belong to D channels each.
 template <int V, bool MSK, bool MOM> struct AdvantageOp {
@@ -370,7 +406,7 @@ template <int V, bool MSK, bool MOM> struct AdvantageOp {
             o.A[v] = in ? (cut ? 0.f : gl) : 1.f;
         }
     }
-    __device__ void step(float (&c)[V], const Item &i, const Lane &l, const Step &s, bool on, double &s1, double &s2, int &cnt) const
+    __device__ void step(float (&c)[V], const Item &i, const Lane &l, const Step &s, bool on, SpreadSum &sum) const
     {
         float oa[V], ov[V];
 #pragma unroll
@@ -379,7 +415,7 @@ template <int V, bool MSK, bool MOM> struct AdvantageOp {
             const bool in = on && (!MSK || s.t() < l.len[v]);
             oa[v] = in ? c[v] : 0.f;
             ov[v] = in ? c[v] + i.val[v] : 0.f;
-            if (MOM && in) { s1 += (double)c[v]; s2 += (double)c[v] * (double)c[v]; ++cnt; }
+            if (MOM && in) sum.add((double)c[v]);
         }
         if (on) {
             put<float, V>(at(adv), step_off(s, C), l.ch * 4u, oa);
@@ -395,7 +431,6 @@ template <class Item> __device__ __forceinline__ bool cut_of(const Item &i, int 
     else return i.cut;
 }
 
-// Moments of the advantages: a partial (count, sum, sum of squares) per workgroup in double, summed in a fixed order.
 __device__ __forceinline__ double wave_sum(double x)
 {
 #pragma unroll
@@ -483,8 +518,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
                 for (int v = 0; v < V; ++v) c[v] = through<CUTS>(ex[0][k][0][lane][v], ex[0][k][1][lane][v], c[v]);
         }
     }
-    double s1 = 0, s2 = 0;
-    int cnt = 0;
+    SpreadSum sum;                                                      // (moments: of this thread's values)
     int par = 1;                                                        // (the half the stretches were not left in)
     // FULL: every step of the tile lies inside the stretch.  NEXT: the next tile is 0 none, 1 perhaps partly beyond the end, 2 full.
     auto work = [&](auto full, auto next, int tile) __attribute__((always_inline)) {
@@ -540,7 +574,7 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
 #pragma unroll
                     for (int v = 0; v < V; ++v) front[v] = l == 0 || l == kept ? mine[v] : front[v];
                 }
-                if constexpr (Op::SUMS) op.step(mine, it[l], ln, step_at(u0, l), on, s1, s2, cnt);
+                if constexpr (Op::SUMS) op.step(mine, it[l], ln, step_at(u0, l), on, sum);
                 else op.step(mine, it[l], ln, step_at(u0, l), on);
             }
             if constexpr (Op::KEEPS) {
@@ -568,13 +602,14 @@ __global__ __launch_bounds__(64 * NW) void k_scan(Op op, ScanGeom q, double *mom
     if (have && wave == 0 && split == q.nsplit - 1) op.finish(c, w.ch);
     if constexpr (Op::MOMENTS) {
         __shared__ double red[NW][3];
-        const double w1 = wave_sum(s1), w2 = wave_sum(s2), w0 = wave_sum((double)cnt);
-        if (lane == 0) { red[wave][0] = w0; red[wave][1] = w1; red[wave][2] = w2; }
+        const Spread ws = wave_join(sum.spread());
+        if (lane == 0) { red[wave][0] = ws.n; red[wave][1] = ws.mean; red[wave][2] = ws.m2; }
         __syncthreads();
-        if (threadIdx.x < 3) {
-            double t = 0;
-            for (int k = 0; k < NW; ++k) t += red[k][threadIdx.x];
-            mom[((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 3 + threadIdx.x] = t;
+        if (threadIdx.x == 0) {
+            Spread t = ws;
+            for (int k = 1; k < NW; ++k) t = join(t, {red[k][0], red[k][1], red[k][2]});
+            double *to = mom + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 3;
+            to[0] = t.n; to[1] = t.mean; to[2] = t.m2;
         }
     }
 }
@@ -664,22 +699,15 @@ __global__ __launch_bounds__(64) void k_scan_back_kept(BackwardKeptOp<T, V, MSK,
 __global__ __launch_bounds__(256) void k_moments(const double *mom, int64_t n, float *out)
 {
     __shared__ double red[4][3];
-    double s[3] = {0, 0, 0};
-    for (int64_t k = threadIdx.x; k < n; k += 256)
-#pragma unroll
-        for (int j = 0; j < 3; ++j) s[j] += mom[k * 3 + j];
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        const double t = wave_sum(s[j]);
-        if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][j] = t;
-    }
+    Spread s{0, 0, 0};
+    for (int64_t k = threadIdx.x; k < n; k += 256) s = join(s, {mom[k * 3], mom[k * 3 + 1], mom[k * 3 + 2]});
+    s = wave_join(s);
+    if ((threadIdx.x & 63) == 0) { red[threadIdx.x >> 6][0] = s.n; red[threadIdx.x >> 6][1] = s.mean; red[threadIdx.x >> 6][2] = s.m2; }
     __syncthreads();
     if (threadIdx.x == 0) {
-        double t[3];
-        for (int j = 0; j < 3; ++j) t[j] = red[0][j] + red[1][j] + red[2][j] + red[3][j];
-        const double k = t[0] > 0 ? t[0] : 1.0, mean = t[1] / k, var = t[2] / k - mean * mean;
-        out[0] = (float)mean;
-        out[1] = (float)(1.0 / (sqrt(var > 0 ? var : 0.0) + 1e-8));
+        for (int k = 1; k < 4; ++k) s = join(s, {red[k][0], red[k][1], red[k][2]});
+        out[0] = (float)s.mean;
+        out[1] = (float)(1.0 / (sqrt(s.n > 0.0 ? s.m2 / s.n : 0.0) + 1e-8));
     }
 }
 
