@@ -20,7 +20,7 @@ struct ScanArgs {
     const int *lengths;
     SeqOut out, dgate, dx;          // out: h of the forward pass
     float *h_last, *dh0;
-    float *kept;                    // the states in front of every eighth step (nullable): written forward, read backward
+    float *kept;                    // the states in front of every eighth step from the end (nullable): written forward, read backward
     void *ws;
 };
 

@@ -380,14 +380,17 @@ class ClippedPolicyLearner:
 def _over_ranks(moments: torch.Tensor, sizes, group) -> torch.Tensor:
     """The moments of all ranks' advantages from each rank's own, and a check that all ranks train on as much, in one message: ranks
     with other numbers of updates would wait for each other for good."""
-    mean, sd = moments[0].double(), 1.0 / moments[1].double() - 1e-8
+    world, rank, k = dist.get_world_size(group), dist.get_rank(group), len(sizes)
     own = torch.tensor([float(s) for s in sizes], dtype=torch.float64, device=moments.device)
-    v = all_reduce_sum(torch.cat((own, own * own, torch.stack((mean, mean * mean + sd * sd)))), group)
-    world, host, k = dist.get_world_size(group), v.tolist(), len(sizes)
+    each = torch.zeros(world, 2, dtype=torch.float64, device=moments.device)        # (a row of its own for each rank: the SUM gathers them)
+    each[rank, 0], each[rank, 1] = moments[0], 1.0 / moments[1].double() - 1e-8
+    v = all_reduce_sum(torch.cat((own, own * own, each.view(-1))), group)
+    host = v[:2 * k].tolist()
     if any(world * sq != s * s for s, sq in zip(host[:k], host[k:2 * k])):      # (equal exactly where all ranks' numbers are)
         raise RuntimeError("train_on_policy: the ranks differ in episode length, environments, agents, epochs or envs_per_batch")
-    mean, square = v[-2] / world, v[-1] / world
-    return torch.stack((mean, 1.0 / ((square - mean * mean).clamp_min(0.0).sqrt() + 1e-8))).float()
+    means, sds = v[2 * k:].view(world, 2).unbind(1)
+    mean = means.mean()
+    return torch.stack((mean, 1.0 / ((sds.square() + (means - mean).square()).mean().sqrt() + 1e-8))).float()
 
 
 def train_on_policy(env: BatchedAssemblyEnv, learner: ClippedPolicyLearner, replay: DeviceReplay, epochs: int = 4, envs_per_batch: int = 64):

@@ -89,10 +89,14 @@ def _worker(rank, world, port, out):
         rollout.train_on_policy(env, alone, replay, epochs=1)
     except RuntimeError as e:
         refused.append(str(e))
+    same = rollout._over_ranks(torch.tensor([777.7, 1e8]), (1,), None)      # (equal everywhere: no deviation appears)
+    assert same.tolist() == torch.tensor([777.7, 1e8]).tolist()
+    two = rollout._over_ranks(torch.tensor([5.0 + rank, 1 / (2.0 + 1e-8)]), (1,), None)
+    assert two.tolist() == pytest.approx([5.5, 1 / (4.25 ** 0.5 + 1e-8)], rel=1e-6)
     own = [dist.new_group([r]) for r in range(world)][rank]
     _, single = _learner(group=own)                                   # a group of this rank alone: nothing to drift from
     rollout.train_on_policy(env, single, replay, epochs=1)
-    out.put((rank, _weights(L), calls == [12] + sizes * EPOCHS, refused))
+    out.put((rank, _weights(L), calls == [10 + 2 * world] + sizes * EPOCHS, refused))
     dist.barrier()
     dist.destroy_process_group()
 
